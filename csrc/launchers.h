@@ -242,3 +242,118 @@ void launch_packed_to_native(const uint8_t* values, const uint64_t* bitmap, cons
                              const int32_t* rows, const int32_t* positions, const float* freqs, int64_t freq_rows,
                              uint8_t* out, const int64_t* dst, int64_t out_slots, int keep, int n, int* err,
                              cudaStream_t stream);
+
+int make_tmap_16b_sw128(void* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                        const uint32_t* box, int half);
+
+// Residual add + RMSNorm -> MXFP8 rows (csrc/norm_mx.cu).  n is a multiple of 32, at most 8192; rows start on
+// 16-byte boundaries; strides in elements; half: x, d, x_out, h are FP16, else BF16.
+struct NormMxArgs {
+  int64_t rows;
+  int n, half;
+  const void* x;
+  int64_t xs;
+  const void* d;      // optional addend of x's type
+  int64_t ds;
+  const float* df;    // optional fp32 addend
+  int64_t dfs;
+  void* x_out;        // the sum in x's type; null: no addend
+  int64_t xos;
+  const float* w;
+  float eps;
+  void* h;            // [rows, n], optional
+  uint8_t* codes;     // [rows, n]
+  uint8_t* scales;    // [rows, n / 32]
+};
+void launch_add_rmsnorm_mx(const NormMxArgs& a, cudaStream_t stream);
+
+// Gradient of residual add + RMSNorm: x is the stored stream.
+struct NormBwdArgs {
+  int64_t rows;
+  int n, half;
+  const void* x;
+  int64_t xs;
+  const void* dh;
+  int64_t dhs;
+  const void* dres;   // gradient of the stream itself, optional
+  int64_t drs;
+  const float* w;
+  float eps;
+  void* dx;           // [rows, n]
+  float* dxf;         // [rows, n], optional: dx before its rounding
+  float* part;        // workspace [slots, n]
+  float* dw;          // [n]
+};
+int rmsnorm_bwd_slots(int64_t rows, int n, int num_sms);
+void launch_rmsnorm_bwd(const NormBwdArgs& a, int slots, cudaStream_t stream);
+
+// Token rows sorted by expert and back (csrc/expert_dispatch.cu).
+int launch_expert_order(const void* ids, bool wide, int64_t id_stride, int64_t T, int k, int64_t base, int E,
+                        int32_t* offsets, int32_t* slots, int32_t* pairs, cudaStream_t stream);
+struct GatherArgs {
+  int64_t T;
+  int k, E, num_sms;
+  const int32_t* slots;
+  const int32_t* offsets;
+  const void* src;        // T rows, src_stride bytes apart
+  int64_t src_stride, row_bytes;
+  void* dst;              // [T k] rows of row_bytes
+  const void* scales;     // optional second plane, the same way
+  int64_t scales_stride, scale_bytes;
+  void* scales_dst;
+};
+void launch_expert_gather(const GatherArgs& a, cudaStream_t stream);
+struct CombineArgs {
+  int64_t T;
+  int k, width, num_sms;
+  const int32_t* slots;
+  const float* weights;   // [T, k] rows ws apart; null: 1
+  int64_t ws;
+  const void* y;
+  int64_t ys;
+  const void* residual;   // optional, the output's type
+  int64_t rs;
+  void* out;              // [T, width]
+};
+struct CombineBwdArgs {
+  int64_t T;
+  int k, width, E;
+  const int32_t* slots;
+  const int32_t* offsets;
+  const float* weights;
+  int64_t ws;
+  const void* y;
+  int64_t ys;
+  const void* dout;
+  int64_t gs;
+  void* dy;               // [T k, width], optional
+  float* dw;              // [T, k], optional
+};
+void launch_expert_combine(const CombineArgs& a, int type, bool out_f32, bool vec, cudaStream_t stream);
+void launch_expert_combine_bwd(const CombineBwdArgs& a, int type, bool out_f32, bool vec, cudaStream_t stream);
+
+// Matrix products of every expert's rows (csrc/expert_mm.cu).
+struct ExpertMmArgs {
+  int E, P, N, M;         // N: output row stride (kForward gated: 2 I); M: output rows of an expert (kGradW)
+  int nk, tiles_m, tiles_n, num_sms, half;
+  const int32_t* offsets;
+  void* out;
+  void* pre;
+  int* err;
+};
+struct ExpertMmCall {
+  const void* x;          // [P, K], rows xs elements apart
+  int64_t xs;
+  const void* w;          // [E, N, K]
+  const void* dz;         // [P, N], rows dzs apart
+  int64_t dzs;
+  const int32_t* offsets; // [E + 1]
+  void* out;
+  void* pre;              // gated forward: the products [P, N], optional
+  int64_t P;
+  int K, N, E, gated, half, num_sms;
+  int* err;
+};
+int launch_expert_mm(int mode, const ExpertMmCall& c, cudaStream_t stream);
+void launch_swiglu_bwd(const void* da, int64_t das, const void* z, int64_t zs, void* dz, int64_t P, int I,
+                       const int32_t* offsets, int E, int half, int num_sms, cudaStream_t stream);

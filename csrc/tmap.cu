@@ -87,3 +87,23 @@ int make_tmap_u8_sw128(void* out, const void* base, uint64_t k_elems, uint64_t r
                  dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
+
+// Tiled map over a 16-bit matrix stack (`rank` <= 5 dims, innermost contiguous, strides in bytes for dims
+// 1..rank-1) with the 128-byte swizzle; box[0] is 64 elements (128 bytes).  Elements outside read as zero.
+int make_tmap_16b_sw128(void* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                        const uint32_t* box, int half) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return -1;
+  cuuint64_t d[5], st[4];
+  cuuint32_t b[5], e[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    e[i] = 1;
+    if (i) st[i - 1] = strides[i - 1];
+  }
+  return (int)fn(reinterpret_cast<CUtensorMap*>(out),
+                 half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank,
+                 const_cast<void*>(base), d, st, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}

@@ -833,8 +833,11 @@ void fp4_store(torch::Tensor raw, torch::Tensor weight, double eps, torch::Tenso
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
+void bind_block_ops(pybind11::module_& m);  // csrc/torch_ops_block.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "packmla sm_100a kernels";
+  bind_block_ops(m);
   m.def("native_store", &native_store, "FP32 rows -> Native 584 B C4 records (paged)");
   m.def("packed_store", &packed_store, "FP32 rows -> Packed 328 B C4 records (planes)");
   m.def("umma_probe", &umma_probe, "tcgen05 operand-layout self-test (one MMA)");

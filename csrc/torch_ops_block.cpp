@@ -1,0 +1,373 @@
+// Torch-facing wrappers of the mixture-of-experts block operators (norm_mx.cu, expert_dispatch.cu,
+// expert_mm.cu): argument validation, output allocation, then the plain launchers.
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include <string>
+
+#include "launchers.h"
+
+namespace {
+using torch::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+cudaStream_t stream() { return at::cuda::getCurrentCUDAStream(); }
+int sms(const Tensor& t) { return at::cuda::getDeviceProperties(t.get_device())->multiProcessorCount; }
+bool is16(const Tensor& t) { return t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kFloat16; }
+bool on16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+// a row of a two-dimensional tensor that has one row may report any stride
+int64_t row_stride(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stride(0); }
+
+// Numbers in messages go through std::to_string: c10::str streams integers, which crashes where the extension
+// and torch were linked with different C++ runtimes.
+std::string num(int64_t v) { return std::to_string(v); }
+
+void check_device(const Tensor& like, const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", like.device());
+}
+void check_rows(const Tensor& like, const Tensor& t, int64_t rows, int64_t n, torch::ScalarType type, const char* name) {
+  check_device(like, t, name);
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == n, name, " must be [", num(rows), ", ", num(n), "]");
+  TORCH_CHECK(t.scalar_type() == type, name, " must be ", type);
+  TORCH_CHECK(t.numel() == 0 || t.stride(1) == 1, name, " rows must be contiguous");
+}
+void check_rows16(const Tensor& like, const Tensor& t, int64_t rows, int64_t n, torch::ScalarType type, const char* name) {
+  check_rows(like, t, rows, n, type, name);
+  TORCH_CHECK(t.numel() == 0 || (on16(t) && row_stride(t) * t.element_size() % 16 == 0), name,
+              " rows must start on 16-byte boundaries");
+}
+void check_weight(const Tensor& like, const Tensor& w, int64_t n) {
+  check_device(like, w, "w");
+  TORCH_CHECK(w.scalar_type() == torch::kFloat32 && w.dim() == 1 && w.size(0) == n && w.is_contiguous() && on16(w),
+              "w must be contiguous fp32 [", num(n), "]");
+}
+void check_norm(const Tensor& x, const char* op) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && is16(x), op, ": x must be a CUDA BF16 or FP16 [rows, n] tensor");
+  TORCH_CHECK(x.size(1) >= 32 && x.size(1) % 32 == 0 && x.size(1) <= 8192, op,
+              ": n must be a multiple of 32 and at most 8192");
+}
+}  // namespace
+
+// -> (stream, codes, scales, h or None); stream is x itself without addends or in place
+std::tuple<Tensor, Tensor, Tensor, OptTensor> add_rmsnorm_mx(const Tensor& x, const Tensor& w, double eps,
+                                                             const OptTensor& d, const OptTensor& df, bool inplace,
+                                                             bool return_h) {
+  check_norm(x, "add_rmsnorm_mx");
+  const int64_t rows = x.size(0), n = x.size(1);
+  check_rows16(x, x, rows, n, x.scalar_type(), "x");
+  check_weight(x, w, n);
+  if (d) check_rows16(x, *d, rows, n, x.scalar_type(), "d");
+  if (df) check_rows16(x, *df, rows, n, torch::kFloat32, "dfp32");
+  const c10::cuda::CUDAGuard g(x.device());
+  const bool add = d || df;
+  Tensor s = add && !inplace ? torch::empty({rows, n}, x.options()) : x;
+  Tensor codes = torch::empty({rows, n}, x.options().dtype(torch::kUInt8));
+  Tensor scales = torch::empty({rows, n / 32}, x.options().dtype(torch::kUInt8));
+  OptTensor h;
+  if (return_h) h = torch::empty({rows, n}, x.options());
+  NormMxArgs a{};
+  a.rows = rows;
+  a.n = (int)n;
+  a.half = x.scalar_type() == torch::kFloat16;
+  a.x = x.data_ptr();
+  a.xs = row_stride(x);
+  if (d) { a.d = d->data_ptr(); a.ds = row_stride(*d); }
+  if (df) { a.df = df->data_ptr<float>(); a.dfs = row_stride(*df); }
+  if (add) { a.x_out = s.data_ptr(); a.xos = row_stride(s); }
+  a.w = w.data_ptr<float>();
+  a.eps = (float)eps;
+  if (h) a.h = h->data_ptr();
+  a.codes = codes.data_ptr<uint8_t>();
+  a.scales = scales.data_ptr<uint8_t>();
+  launch_add_rmsnorm_mx(a, stream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {s, codes, scales, h};
+}
+
+// -> (dx in x's type, dw fp32, dx in fp32 or None)
+std::tuple<Tensor, Tensor, OptTensor> rmsnorm_backward(const Tensor& dh, const Tensor& x, const Tensor& w, double eps,
+                                                       const OptTensor& dres, bool fp32_dx) {
+  check_norm(x, "add_rmsnorm_backward");
+  const int64_t rows = x.size(0), n = x.size(1);
+  check_rows16(x, x, rows, n, x.scalar_type(), "x");
+  check_rows16(x, dh, rows, n, x.scalar_type(), "dh");
+  check_weight(x, w, n);
+  if (dres) check_rows16(x, *dres, rows, n, x.scalar_type(), "dres");
+  const c10::cuda::CUDAGuard g(x.device());
+  const int slots = rmsnorm_bwd_slots(rows, (int)n, sms(x));
+  const auto f32 = x.options().dtype(torch::kFloat32);
+  Tensor dx = torch::empty({rows, n}, x.options()), dw = torch::empty({n}, f32);
+  Tensor part = torch::empty({slots, n}, f32);
+  OptTensor dxf;
+  if (fp32_dx) dxf = torch::empty({rows, n}, f32);
+  NormBwdArgs a{};
+  a.rows = rows;
+  a.n = (int)n;
+  a.half = x.scalar_type() == torch::kFloat16;
+  a.x = x.data_ptr();
+  a.xs = row_stride(x);
+  a.dh = dh.data_ptr();
+  a.dhs = row_stride(dh);
+  if (dres) { a.dres = dres->data_ptr(); a.drs = row_stride(*dres); }
+  a.w = w.data_ptr<float>();
+  a.eps = (float)eps;
+  a.dx = dx.data_ptr();
+  if (dxf) a.dxf = dxf->data_ptr<float>();
+  a.part = part.data_ptr<float>();
+  a.dw = dw.data_ptr<float>();
+  launch_rmsnorm_bwd(a, slots, stream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {dx, dw, dxf};
+}
+
+// -> (offsets [E + 1], slots [T, k], pairs [T k])
+std::tuple<Tensor, Tensor, Tensor> expert_order(const Tensor& ids, int64_t num_experts, int64_t expert_base) {
+  TORCH_CHECK(ids.is_cuda() && ids.dim() == 2 &&
+              (ids.scalar_type() == torch::kInt32 || ids.scalar_type() == torch::kInt64),
+              "expert_order: ids must be a CUDA int32 or int64 [tokens, topk] tensor");
+  TORCH_CHECK(num_experts >= 1 && num_experts <= 4096, "expert_order: num_experts must be in [1, 4096]");
+  TORCH_CHECK(ids.numel() == 0 || ids.size(1) == 1 || ids.stride(1) == 1, "expert_order: a token's ids must be contiguous");
+  TORCH_CHECK(ids.numel() < (1 << 30), "expert_order: at most 2^30 pairs");
+  const c10::cuda::CUDAGuard g(ids.device());
+  const int64_t T = ids.size(0), k = ids.size(1);
+  const auto i32 = ids.options().dtype(torch::kInt32);
+  if (T * k == 0) return {torch::zeros({num_experts + 1}, i32), torch::empty({T, k}, i32), torch::empty({0}, i32)};
+  Tensor offsets = torch::empty({num_experts + 1}, i32), slots = torch::empty({T, k}, i32), pairs = torch::empty({T * k}, i32);
+  const int rc = launch_expert_order(ids.data_ptr(), ids.scalar_type() == torch::kInt64, T == 1 ? k : ids.stride(0), T,
+                                     (int)k, expert_base, (int)num_experts, offsets.data_ptr<int32_t>(),
+                                     slots.data_ptr<int32_t>(), pairs.data_ptr<int32_t>(), stream());
+  TORCH_CHECK(rc == 0, "expert_order: launch failed (", num(rc), ")");
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {offsets, slots, pairs};
+}
+
+namespace {
+void check_order(const Tensor& like, const Tensor& offsets, const Tensor& slots) {
+  check_device(like, offsets, "offsets");
+  check_device(like, slots, "slots");
+  TORCH_CHECK(offsets.scalar_type() == torch::kInt32 && offsets.dim() == 1 && offsets.size(0) >= 2 &&
+              offsets.is_contiguous(), "offsets must be contiguous int32 [experts + 1]");
+  TORCH_CHECK(slots.scalar_type() == torch::kInt32 && slots.dim() == 2 && slots.is_contiguous(),
+              "slots must be contiguous int32 [tokens, topk]");
+}
+}  // namespace
+
+// x [T, width] (and scales [T, ...], uint8) -> the same for the sorted rows
+std::tuple<Tensor, OptTensor> expert_gather(const Tensor& x, const OptTensor& scales, const Tensor& slots,
+                                            const Tensor& offsets) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2, "gather: x must be a CUDA [tokens, width] tensor");
+  check_order(x, offsets, slots);
+  const int64_t T = slots.size(0), k = slots.size(1);
+  check_rows(x, x, T, x.size(1), x.scalar_type(), "x");
+  if (scales) check_rows(x, *scales, T, scales->size(1), torch::kUInt8, "scales");
+  const c10::cuda::CUDAGuard g(x.device());
+  Tensor out = torch::empty({T * k, x.size(1)}, x.options());
+  OptTensor sout;
+  if (scales) sout = torch::empty({T * k, scales->size(1)}, scales->options());
+  GatherArgs a{};
+  a.T = T;
+  a.k = (int)k;
+  a.E = (int)offsets.size(0) - 1;
+  a.num_sms = sms(x);
+  a.slots = slots.data_ptr<int32_t>();
+  a.offsets = offsets.data_ptr<int32_t>();
+  a.src = x.data_ptr();
+  a.row_bytes = x.size(1) * x.element_size();
+  a.src_stride = row_stride(x) * x.element_size();
+  a.dst = out.data_ptr();
+  if (scales && scales->size(1) > 0) {
+    a.scales = scales->data_ptr();
+    a.scale_bytes = scales->size(1);
+    a.scales_stride = row_stride(*scales);
+    a.scales_dst = sout->data_ptr();
+  }
+  launch_expert_gather(a, stream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {out, sout};
+}
+
+namespace {
+int row_type(const Tensor& y, const char* op) {
+  TORCH_CHECK(y.is_cuda() && y.dim() == 2 && (is16(y) || y.scalar_type() == torch::kFloat32), op,
+              ": rows must be a CUDA BF16, FP16 or FP32 [rows, width] tensor");
+  return y.scalar_type() == torch::kFloat32 ? 2 : y.scalar_type() == torch::kFloat16 ? 1 : 0;
+}
+bool wide(const Tensor& t) { return t.size(1) % 8 == 0 && on16(t) && row_stride(t) * t.element_size() % 16 == 0; }
+}  // namespace
+
+Tensor expert_combine(const Tensor& y, const OptTensor& weights, const OptTensor& residual, const Tensor& slots,
+                      const Tensor& offsets, bool out_f32) {
+  const int type = row_type(y, "combine");
+  check_order(y, offsets, slots);
+  const int64_t T = slots.size(0), k = slots.size(1), width = y.size(1);
+  check_rows(y, y, T * k, width, y.scalar_type(), "y");
+  const auto out_type = out_f32 ? torch::kFloat32 : y.scalar_type();
+  if (weights) check_rows(y, *weights, T, k, torch::kFloat32, "weights");
+  if (residual) check_rows(y, *residual, T, width, out_type, "residual");
+  const c10::cuda::CUDAGuard g(y.device());
+  Tensor out = torch::empty({T, width}, y.options().dtype(out_type));
+  CombineArgs a{};
+  a.T = T;
+  a.k = (int)k;
+  a.width = (int)width;
+  a.num_sms = sms(y);
+  a.slots = slots.data_ptr<int32_t>();
+  if (weights) { a.weights = weights->data_ptr<float>(); a.ws = row_stride(*weights); }
+  a.y = y.data_ptr();
+  a.ys = row_stride(y);
+  if (residual) { a.residual = residual->data_ptr(); a.rs = row_stride(*residual); }
+  a.out = out.data_ptr();
+  launch_expert_combine(a, type, out_f32, wide(y) && (!residual || wide(*residual)), stream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return out;
+}
+
+// -> (dy or None, dweights or None)
+std::tuple<OptTensor, OptTensor> expert_combine_backward(const Tensor& dout, const Tensor& y, const Tensor& weights,
+                                                         const Tensor& slots, const Tensor& offsets, bool need_dy,
+                                                         bool need_dw) {
+  const int type = row_type(y, "combine_backward");
+  check_order(y, offsets, slots);
+  const int64_t T = slots.size(0), k = slots.size(1), width = y.size(1);
+  check_rows(y, y, T * k, width, y.scalar_type(), "y");
+  check_rows(y, weights, T, k, torch::kFloat32, "weights");
+  TORCH_CHECK(dout.scalar_type() == y.scalar_type() || dout.scalar_type() == torch::kFloat32,
+              "combine_backward: dout must be fp32 or have y's type");
+  check_rows(y, dout, T, width, dout.scalar_type(), "dout");
+  const c10::cuda::CUDAGuard g(y.device());
+  OptTensor dy, dw;
+  if (need_dy) dy = torch::empty({T * k, width}, y.options());
+  if (need_dw) dw = torch::empty({T, k}, weights.options());
+  CombineBwdArgs a{};
+  a.T = T;
+  a.k = (int)k;
+  a.width = (int)width;
+  a.E = (int)offsets.size(0) - 1;
+  a.slots = slots.data_ptr<int32_t>();
+  a.offsets = offsets.data_ptr<int32_t>();
+  a.weights = weights.data_ptr<float>();
+  a.ws = row_stride(weights);
+  a.y = y.data_ptr();
+  a.ys = row_stride(y);
+  a.dout = dout.data_ptr();
+  a.gs = row_stride(dout);
+  if (dy) a.dy = dy->data_ptr();
+  if (dw) a.dw = dw->data_ptr<float>();
+  if (need_dy || need_dw)
+    launch_expert_combine_bwd(a, type, dout.scalar_type() == torch::kFloat32, wide(y) && wide(dout), stream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {dy, dw};
+}
+
+namespace {
+void check_mm(const Tensor& w, const Tensor& offsets, const Tensor& err, const char* op) {
+  TORCH_CHECK(w.is_cuda() && w.dim() == 3 && is16(w), op, ": w must be a CUDA BF16 or FP16 [experts, n, k] tensor");
+  TORCH_CHECK(w.is_contiguous() && on16(w), op, ": w must be contiguous and start on a 16-byte boundary");
+  TORCH_CHECK(w.size(0) >= 1 && w.size(0) <= 1024, op, ": 1 to 1024 experts");
+  TORCH_CHECK(w.size(1) >= 8 && w.size(1) % 8 == 0 && w.size(2) >= 8 && w.size(2) % 8 == 0, op,
+              ": n and k must be multiples of 8");
+  check_device(w, offsets, "offsets");
+  TORCH_CHECK(offsets.scalar_type() == torch::kInt32 && offsets.dim() == 1 && offsets.size(0) == w.size(0) + 1 &&
+              offsets.is_contiguous(), op, ": offsets must be contiguous int32 [experts + 1]");
+  check_device(w, err, "err");
+  TORCH_CHECK(err.scalar_type() == torch::kInt32 && err.numel() >= 4, "err must be CUDA int32[4]");
+}
+ExpertMmCall mm_call(const Tensor& w, const Tensor& offsets, const Tensor& err, int64_t P) {
+  TORCH_CHECK(P < (1 << 30), "at most 2^30 rows");
+  ExpertMmCall c{};
+  c.w = w.data_ptr();
+  c.offsets = offsets.data_ptr<int32_t>();
+  c.P = P;
+  c.E = (int)w.size(0);
+  c.N = (int)w.size(1);
+  c.K = (int)w.size(2);
+  c.half = w.scalar_type() == torch::kFloat16;
+  c.num_sms = sms(w);
+  c.err = err.data_ptr<int>();
+  return c;
+}
+void run_mm(int mode, const ExpertMmCall& c) {
+  const int rc = launch_expert_mm(mode, c, stream());
+  TORCH_CHECK(rc == 0, "expert products: tensor map or shared memory refused (", num(rc), ")");
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+}  // namespace
+
+// -> (y, the products z or None); gated: y = silu(z[:, :n / 2]) z[:, n / 2:]
+std::tuple<Tensor, OptTensor> expert_mm(const Tensor& x, const Tensor& w, const Tensor& offsets, bool gated,
+                                        bool save_pre, const Tensor& err) {
+  check_mm(w, offsets, err, "expert_linear");
+  const int64_t P = x.size(0), N = w.size(1), K = w.size(2);
+  check_rows16(w, x, P, K, w.scalar_type(), "x");
+  TORCH_CHECK(!gated || N % 16 == 0, "expert_linear: a gated product needs n a multiple of 16");
+  TORCH_CHECK(gated || !save_pre, "expert_linear: only a gated product keeps its operands");
+  const c10::cuda::CUDAGuard g(w.device());
+  Tensor y = torch::empty({P, gated ? N / 2 : N}, x.options());
+  OptTensor pre;
+  if (save_pre) pre = torch::empty({P, N}, x.options());
+  if (P > 0) {
+    ExpertMmCall c = mm_call(w, offsets, err, P);
+    c.x = x.data_ptr();
+    c.xs = row_stride(x);
+    c.out = y.data_ptr();
+    c.pre = pre ? pre->data_ptr() : nullptr;
+    c.gated = gated;
+    run_mm(0, c);
+  }
+  return {y, pre};
+}
+
+// -> (dx or None, dw or None)
+std::tuple<OptTensor, OptTensor> expert_mm_backward(const Tensor& dz, const Tensor& x, const Tensor& w,
+                                                    const Tensor& offsets, bool need_dx, bool need_dw,
+                                                    const Tensor& err) {
+  check_mm(w, offsets, err, "expert_linear_backward");
+  const int64_t P = x.size(0), N = w.size(1), K = w.size(2);
+  check_rows16(w, x, P, K, w.scalar_type(), "x");
+  check_rows16(w, dz, P, N, w.scalar_type(), "dy");
+  const c10::cuda::CUDAGuard g(w.device());
+  OptTensor dx, dw;
+  if (need_dx) dx = torch::empty({P, K}, x.options());
+  if (need_dw) dw = P > 0 ? torch::empty_like(w) : torch::zeros_like(w);
+  if (P > 0) {
+    ExpertMmCall c = mm_call(w, offsets, err, P);
+    c.x = x.data_ptr();
+    c.xs = row_stride(x);
+    c.dz = dz.data_ptr();
+    c.dzs = row_stride(dz);
+    if (dx) { c.out = dx->data_ptr(); run_mm(1, c); }
+    if (dw) { c.out = dw->data_ptr(); run_mm(2, c); }
+  }
+  return {dx, dw};
+}
+
+Tensor swiglu_backward(const Tensor& da, const Tensor& pre, const Tensor& offsets) {
+  TORCH_CHECK(pre.is_cuda() && pre.dim() == 2 && is16(pre) && pre.size(1) >= 16 && pre.size(1) % 16 == 0,
+              "swiglu_backward: pre must be a CUDA BF16 or FP16 [rows, n] tensor, n a multiple of 16");
+  const int64_t P = pre.size(0), N = pre.size(1);
+  check_rows16(pre, pre, P, N, pre.scalar_type(), "pre");
+  check_rows16(pre, da, P, N / 2, pre.scalar_type(), "dy");
+  check_device(pre, offsets, "offsets");
+  TORCH_CHECK(offsets.scalar_type() == torch::kInt32 && offsets.dim() == 1 && offsets.size(0) >= 2 &&
+              offsets.is_contiguous(), "swiglu_backward: offsets must be contiguous int32 [experts + 1]");
+  const c10::cuda::CUDAGuard g(pre.device());
+  Tensor dz = torch::empty({P, N}, pre.options());
+  launch_swiglu_bwd(da.data_ptr(), row_stride(da), pre.data_ptr(), row_stride(pre), dz.data_ptr(), P, (int)(N / 2),
+                    offsets.data_ptr<int32_t>(), (int)offsets.size(0) - 1, pre.scalar_type() == torch::kFloat16,
+                    sms(pre), stream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return dz;
+}
+
+void bind_block_ops(pybind11::module_& m) {
+  m.def("add_rmsnorm_mx", &add_rmsnorm_mx, "residual add + RMSNorm -> MXFP8 rows");
+  m.def("rmsnorm_backward", &rmsnorm_backward, "gradient of residual add + RMSNorm");
+  m.def("expert_order", &expert_order, "stable sort of (token, choice) pairs by expert");
+  m.def("expert_gather", &expert_gather, "token rows -> rows sorted by expert");
+  m.def("expert_combine", &expert_combine, "rows sorted by expert -> weighted sums per token");
+  m.def("expert_combine_backward", &expert_combine_backward, "gradients of expert_combine");
+  m.def("expert_mm", &expert_mm, "every expert's matrix product (tcgen05), optionally gated");
+  m.def("expert_mm_backward", &expert_mm_backward, "gradients of expert_mm (tcgen05)");
+  m.def("swiglu_backward", &swiglu_backward, "gradient of silu(gate) * up over sorted rows");
+}

@@ -3,8 +3,9 @@ from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
-from ..formats import abi
+from ..formats import abi, codec
 from ._ext import ext
 
 
@@ -92,3 +93,124 @@ def silu_mul(gu: torch.Tensor) -> torch.Tensor:
         ext().silu_mul(gu, out)
         return out
     return (F.silu(gu[:, :I].float()) * gu[:, I:].float()).to(torch.bfloat16)
+
+
+MX_GROUP = 32  # columns that share one UE8M0 scale of an MXFP8 row
+
+
+def _norm_oracle(s: torch.Tensor, w: torch.Tensor, eps: float):
+    """(s r, r) of fp32 rows s: the normalized rows before the weight, and r = (mean(s^2) + eps)^-1/2."""
+    r = torch.rsqrt(s.square().mean(-1, keepdim=True) + eps)
+    return s * r, r
+
+
+def mx_quantize(h: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """fp32 rows [T, n] -> (E4M3 codes [T, n], UE8M0 scale bytes [T, n / 32]), uint8 (the rule of `mx_dequantize`'s inverse)."""
+    b = h.float().unflatten(-1, (h.shape[1] // MX_GROUP, MX_GROUP))
+    e = codec.ue8m0_exponent(b.abs().amax(-1))
+    return codec.e4m3_encode(b * codec.exp2_int(-e)[..., None]).reshape(h.shape), (e + 127).to(torch.uint8)
+
+
+def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """MXFP8 rows -> code x 2^(scale - 127).  Exact in BF16 and fp32 (E4M3 has four significant bits)."""
+    v = codec.e4m3_decode(codes).unflatten(-1, (codes.shape[1] // MX_GROUP, MX_GROUP))
+    return (v * codec.exp2_int(scales.to(torch.int32) - 127)[..., None]).reshape(codes.shape).to(dtype)
+
+
+def _check_norm(x: torch.Tensor, w: torch.Tensor) -> None:
+    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("x must be a BF16 or FP16 [rows, n] tensor")
+    if x.shape[1] % MX_GROUP or not 0 < x.shape[1] <= 8192:
+        raise ValueError(f"n = {x.shape[1]} must be a multiple of {MX_GROUP} and at most 8192")
+    if w.shape != (x.shape[1],) or w.dtype != torch.float32:
+        raise ValueError("w must be fp32 [n]")
+
+
+def _rows16(t: torch.Tensor | None) -> torch.Tensor | None:
+    """`t` itself if its rows are contiguous and start on 16-byte boundaries, else a contiguous copy."""
+    if t is None or (t.stride(1) == 1 and t.stride(0) * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0):
+        return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def _add_rmsnorm_mx(x, w, eps, d, dfp32, inplace, return_h):
+    if x.is_cuda:
+        xr = x if inplace else _rows16(x)
+        s, codes, scales, h = ext().add_rmsnorm_mx(xr, w, float(eps), _rows16(d), _rows16(dfp32), inplace, return_h)
+        return (x if d is None and dfp32 is None else s), codes, scales, h
+    _check_norm(x, w)
+    s = x
+    if d is not None or dfp32 is not None:
+        s = x.float()
+        for t in (d, dfp32):
+            if t is not None:
+                s = s + t.float()
+        s = x.copy_(s) if inplace else s.to(x.dtype)
+    h = _norm_oracle(s.float(), w, eps)[0] * w
+    return (s, *mx_quantize(h), h.to(x.dtype) if return_h else None)
+
+
+def add_rmsnorm_backward(dh: torch.Tensor, x: torch.Tensor, w: torch.Tensor, eps: float,
+                         dres: torch.Tensor | None = None, fp32_dx: bool = False):
+    """Gradients of `add_rmsnorm` / `add_rmsnorm_mx` at the stored stream x, from dh (of h) and dres (of x itself).
+
+    Returns (dx, dw) - dx in x's type is also the gradient of the addend d, dw is fp32 and does not depend on
+    timing (fixed summation order) - or (dx, dw, fp32 dx) with `fp32_dx`, the gradient of the fp32 addend."""
+    if x.is_cuda:
+        dx, dw, dxf = ext().rmsnorm_backward(_rows16(dh), _rows16(x), w, float(eps), _rows16(dres), fp32_dx)
+        return (dx, dw, dxf) if fp32_dx else (dx, dw)
+    _check_norm(x, w)
+    n, r = _norm_oracle(x.float(), w, eps)
+    g = dh.float() * w
+    dxf = r * (g - n * (g * n).mean(-1, keepdim=True))
+    if dres is not None:
+        dxf = dxf + dres.float()
+    dw = (dh.float() * n).sum(0)
+    return (dxf.to(x.dtype), dw, dxf) if fp32_dx else (dxf.to(x.dtype), dw)
+
+
+class _AddRmsNormMx(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, d, dfp32, eps, return_h):
+        s, codes, scales, h = _add_rmsnorm_mx(x, w, eps, d, dfp32, False, return_h)
+        if s is x:
+            s = x.view_as(x)
+        ctx.save_for_backward(s, w)
+        ctx.eps = eps
+        ctx.addends = d is not None, dfp32 is not None
+        ctx.mark_non_differentiable(codes, scales)
+        ctx.set_materialize_grads(False)
+        return s, codes, scales, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, ds, _codes, _scales, dh):
+        s, w = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        has_d, has_f = ctx.addends
+        if dh is None:  # only the stream was used
+            dx, dw, dxf = ds, None, ds.float() if ds is not None and has_f else None
+        else:
+            dx, dw, *rest = add_rmsnorm_backward(dh, s, w, ctx.eps, ds, fp32_dx=has_f and need[3])
+            dxf = rest[0] if rest else None
+        return (dx if need[0] else None, dw if need[1] else None, dx if has_d and need[2] else None,
+                dxf if has_f and need[3] else None, None, None)
+
+
+def add_rmsnorm_mx(x: torch.Tensor, w: torch.Tensor, eps: float, d: torch.Tensor | None = None,
+                   dfp32: torch.Tensor | None = None, inplace: bool = False, return_h: bool = False):
+    """Residual add + RMSNorm with MXFP8 rows out: (x_new, codes, scales, h).
+
+    x_new = x + d + dfp32 in x's type (x itself without an addend; written over x with `inplace`);
+    h = x_new * rsqrt(mean(x_new^2) + eps) * w in fp32; codes [T, n] are the E4M3 codes of h (uint8) and scales
+    [T, n / 32] its UE8M0 scale bytes, one per 32 columns; with `return_h`, h rounded to x's type (the router's and
+    the shared expert's input), else None.  x, d: BF16 or FP16 [T, n], n a multiple of 32 up to 8192; w fp32 [n].
+
+    Differentiable in x, w, d and dfp32 through x_new and h; the codes carry no gradient (a trainer that feeds
+    them to its products uses h's gradient for them)."""
+    wanted = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, d, dfp32))
+    if not wanted:
+        return _add_rmsnorm_mx(x, w, eps, d, dfp32, inplace, return_h)
+    if inplace:
+        raise ValueError("inplace is not available where a gradient is recorded")
+    return _AddRmsNormMx.apply(x, w, d, dfp32, eps, return_h)

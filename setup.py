@@ -13,7 +13,7 @@ from torch.utils.cpp_extension import BuildExtension, CUDAExtension
 
 os.environ.setdefault("TORCH_CUDA_ARCH_LIST", "10.0a")
 ROOT = os.path.dirname(os.path.abspath(__file__))
-SOURCES = sorted(glob.glob(os.path.join("csrc", "*.cu"))) + ["csrc/torch_ops.cpp"]
+SOURCES = sorted(glob.glob(os.path.join("csrc", "*.cu"))) + ["csrc/torch_ops.cpp", "csrc/torch_ops_block.cpp"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
