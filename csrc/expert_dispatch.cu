@@ -12,6 +12,8 @@
 // All but order are bound by HBM: one pass over the rows.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "launchers.h"
 #include "common/sm100.cuh"
 #include "common/rows.cuh"
@@ -21,56 +23,81 @@ namespace cg = cooperative_groups;
 
 // ----------------------------------------------------------------------------- order
 // A stable counting sort in one launch: the CTAs of one cluster (1 to 8) take consecutive ranges of pairs, the
-// warps of a CTA consecutive ranges of its range.  Pass 1 counts per warp (lanes of equal expert found by
-// match_any, one of them adds: no atomics), the counts become starting rows (over experts, then CTAs through
-// distributed shared memory, then warps), pass 2 hands out rows in the same order.
+// warps of a CTA consecutive ranges of its range.  Pass 1 counts per warp (one lane of those with equal experts
+// adds: no atomics), the counts become starting rows (over warps, then CTAs, then experts), pass 2 hands out
+// rows in the same order.  Latency bound: a lane's first kHeld ids and its peers of equal expert stay in
+// registers for both passes, the ids loaded together, and each CTA pushes its counts into the others' shared
+// memory, so that after the cluster barrier all reads are local.
+constexpr int kHeld = 8;  // ids of a lane held in registers (8 x 32 lanes x 16 warps x 16 CTAs = 65536 pairs)
+
 template <typename Id>
-__global__ void __launch_bounds__(1024) expert_order_kernel(const Id* __restrict__ ids, int64_t id_stride, int k,
-                                                            int n, int64_t base, int E, int32_t* __restrict__ offsets,
-                                                            int32_t* __restrict__ slots,
+__global__ void __launch_bounds__(512) expert_order_kernel(const Id* __restrict__ ids, int n, int64_t base, int E,
+                                                            int32_t* __restrict__ offsets, int32_t* __restrict__ slots,
                                                             int32_t* __restrict__ pairs) {
   extern __shared__ int32_t sm[];
   __shared__ int32_t wsum[32];
   const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
-  int32_t* cnt = sm;           // [W][E]: counts, then the next row of (warp, expert)
-  int32_t* tot = sm + W * E;   // [E]: this CTA's counts
-  int32_t* start = tot + E;    // [E]: the expert's first row in this CTA
   cg::cluster_group cl = cg::this_cluster();
   const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
-  for (int i = tid; i < W * E; i += blockDim.x) cnt[i] = 0;
-  __syncthreads();
+  int32_t* cnt = sm;           // [W][E]: counts, then the next row of (warp, expert)
+  int32_t* tot = sm + W * E;   // [C][E]: every CTA's counts
   const int per = (((n + C * W - 1) / (C * W)) + 31) / 32 * 32;  // pairs of a warp
-  const int lo = min((int64_t)n, (int64_t)(rank * W + warp) * per), hi = min((int64_t)n, (int64_t)lo + per);
+  const int lo = (int)min((int64_t)n, (int64_t)(rank * W + warp) * per), hi = (int)min((int64_t)n, (int64_t)lo + per);
   auto expert = [&](int i) -> int {
     if (i >= hi) return -1;
-    const int64_t e = (int64_t)ids[(int64_t)(i / k) * id_stride + i % k] - base;
+    const int64_t e = (int64_t)ids[i] - base;
     return e >= 0 && e < E ? (int)e : -1;
   };
-  for (int i0 = lo; i0 < hi; i0 += 32) {
-    const int e = expert(i0 + lane);
-    const unsigned m = __match_any_sync(0xffffffffu, e);
-    if (e >= 0 && lane == __ffs(m) - 1) cnt[warp * E + e] += __popc(m);
+  int held[kHeld];
+  unsigned peer[kHeld];
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) held[j] = expert(lo + 32 * j + lane);
+  const int bits = 32 - __clz(E);  // of 0 .. E (E: no expert)
+  auto peers = [&](int e) {  // lanes of the same expert
+    const unsigned v = e >= 0 ? (unsigned)e : (unsigned)E;
+    unsigned m = 0xffffffffu;
+#pragma unroll
+    for (int b = 0; b < 8; ++b)  // bits past the last are 0 in every lane: no change
+      m &= __ballot_sync(0xffffffffu, (v >> b) & 1) ^ (((v >> b) & 1) - 1);
+    for (int b = 8; b < bits; ++b) m &= __ballot_sync(0xffffffffu, (v >> b) & 1) ^ (((v >> b) & 1) - 1);
+    return m;
+  };
+  for (int i = tid; i < W * E; i += blockDim.x) cnt[i] = 0;
+  __syncthreads();
+  int32_t* mine = cnt + warp * E;
+  auto count = [&](int e, unsigned m) {
+    if (e >= 0 && lane == __ffs(m) - 1) mine[e] += __popc(m);
     __syncwarp();
+  };
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j)
+    if (lo + 32 * j < hi) count(held[j], peer[j] = peers(held[j]));
+  for (int i0 = lo + 32 * kHeld; i0 < hi; i0 += 32) {
+    const int e = expert(i0 + lane);
+    count(e, peers(e));
   }
   __syncthreads();
   for (int e = tid; e < E; e += blockDim.x) {
-    int run = 0;
-    for (int w = 0; w < W; ++w) {
-      const int c = cnt[w * E + e];
-      cnt[w * E + e] = run;
-      run += c;
-    }
-    tot[e] = run;
+    int c[16], run = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) c[w] = w < W ? cnt[w * E + e] : 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w)
+      if (w < W) {
+        cnt[w * E + e] = run;
+        run += c[w];
+      }
+    for (int r = 0; r < C; ++r) *cl.map_shared_rank(tot + rank * E + e, r) = run;
   }
   cl.sync();
-  // experts' first rows: exclusive sums over E of the clusters' counts, blockDim.x experts at a time
+  // experts' first rows: exclusive sums over E of the cluster's counts, blockDim.x experts at a time
   int carry = 0;
   for (int e0 = 0; e0 < E; e0 += blockDim.x) {
     const int e = e0 + tid;
     int all = 0, before = 0;
     if (e < E)
       for (int c = 0; c < C; ++c) {
-        const int v = C == 1 ? tot[e] : *cl.map_shared_rank(tot + e, c);
+        const int v = tot[c * E + e];
         all += v;
         if (c < rank) before += v;
       }
@@ -82,33 +109,39 @@ __global__ void __launch_bounds__(1024) expert_order_kernel(const Id* __restrict
     }
     if (lane == 31) wsum[warp] = inc;
     __syncthreads();
-    int wbase = 0, block_sum = 0;
-    for (int w = 0; w < W; ++w) {
-      if (w < warp) wbase += wsum[w];
-      block_sum += wsum[w];
+    int ws = lane < W ? wsum[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, ws, o);
+      if (lane >= o) ws += u;
     }
+    const int wbase = warp ? __shfl_sync(0xffffffffu, ws, warp - 1) : 0;
+    const int first = carry + wbase + inc - all;
     if (e < E) {
-      const int first = carry + wbase + inc - all;
-      start[e] = first + before;
+      tot[e] = first + before;  // row 0 of the table: only this thread reads column e
       if (rank == 0) offsets[e] = first;
     }
-    carry += block_sum;
+    carry += __shfl_sync(0xffffffffu, ws, 31);
     __syncthreads();
   }
   if (rank == 0 && tid == 0) offsets[E] = carry;
-  for (int i0 = lo; i0 < hi; i0 += 32) {
-    const int i = i0 + lane, e = expert(i);
-    const unsigned m = __match_any_sync(0xffffffffu, e);
+  auto place = [&](int i, int e, unsigned m) {
     int row = -1;
-    if (e >= 0) row = start[e] + cnt[warp * E + e] + __popc(m & ((1u << lane) - 1));
+    if (e >= 0) row = tot[e] + mine[e] + __popc(m & ((1u << lane) - 1));
     __syncwarp();
-    if (e >= 0 && lane == __ffs(m) - 1) cnt[warp * E + e] += __popc(m);
+    if (e >= 0 && lane == __ffs(m) - 1) mine[e] += __popc(m);
     __syncwarp();
     if (i < hi) slots[i] = row;
     if (row >= 0) pairs[row] = i;
+  };
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j)
+    if (lo + 32 * j < hi) place(lo + 32 * j + lane, held[j], peer[j]);
+  for (int i0 = lo + 32 * kHeld; i0 < hi; i0 += 32) {
+    const int e = expert(i0 + lane);
+    place(i0 + lane, e, peers(e));
   }
   for (int i = carry + rank * blockDim.x + tid; i < n; i += C * blockDim.x) pairs[i] = -1;
-  cl.sync();  // the other CTAs have read this one's counts
 }
 
 // ----------------------------------------------------------------------------- gather
@@ -195,42 +228,82 @@ __device__ __forceinline__ void store_n(T* p, const float (&v)[NV]) {
 
 constexpr int kBatch = 8;  // choices whose rows are in flight together
 
-// Block (token, column part): thread c of the part sums its NV columns over the token's choices.
-template <typename T, typename O, int NV>
-__global__ void __launch_bounds__(256) expert_combine_kernel(const CombineArgs a) {
-  const int64_t t = blockIdx.x;
-  const int nv = a.width / NV;
-  const int32_t* slot = a.slots + t * a.k;
-  const float* wt = a.weights ? a.weights + t * a.ws : nullptr;
-  const T* y = static_cast<const T*>(a.y);
-  for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < nv; c += gridDim.y * blockDim.x) {
-    float acc[NV];
-    if (a.residual)
-      load_n<O, NV>(static_cast<const O*>(a.residual) + t * a.rs + (int64_t)c * NV, acc);
-    else
+// NV consecutive elements as loaded: converted only where they are added, so that kBatch rows in flight cost
+// 4 registers each (16-bit types) instead of 8.
+template <typename T, int NV>
+struct Raw {
+  static constexpr int kWords = NV == 1 ? 1 : NV * (int)sizeof(T) / 16;
+  using Word = std::conditional_t<NV == 1, T, uint4>;
+  Word w[kWords];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) acc[i] = 0.f;
-    for (int j0 = 0; j0 < a.k; j0 += kBatch) {
-      float v[kBatch][NV];
-      float w[kBatch];
+    for (int i = 0; i < kWords; ++i) w[i] = reinterpret_cast<const Word*>(p)[i];
+  }
+  __device__ __forceinline__ void get(float (&v)[NV]) const {
+    if constexpr (NV == 1) {
+      v[0] = rows::to_f<T>(w[0]);
+    } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        const int r = j0 + j < a.k ? slot[j0 + j] : -1;
-        const bool here = has_row(r, a.T * a.k);
-        // a pair without a row adds nothing, whatever its weight holds
-        w[j] = here ? (wt ? wt[j0 + j] : 1.f) : 0.f;
-        if (here)
-          load_n<T, NV>(y + (int64_t)r * a.ys + (int64_t)c * NV, v[j]);
-        else
-#pragma unroll
-          for (int i = 0; i < NV; ++i) v[j][i] = 0.f;
+      for (int i = 0; i < kWords; ++i) {
+        v[4 * i] = __uint_as_float(w[i].x);
+        v[4 * i + 1] = __uint_as_float(w[i].y);
+        v[4 * i + 2] = __uint_as_float(w[i].z);
+        v[4 * i + 3] = __uint_as_float(w[i].w);
       }
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j)
-#pragma unroll
-        for (int i = 0; i < NV; ++i) acc[i] = fmaf(w[j], v[j][i], acc[i]);
+    } else {
+      rows::unpack8<T>(w[0], v);
     }
-    store_n<O, NV>(static_cast<O*>(a.out) + t * (int64_t)a.width + (int64_t)c * NV, acc);
+  }
+};
+
+// Block (tokens [tpb b, tpb (b + 1)), column part): thread c of the part sums its NV columns over each token's
+// choices.  The tokens' slots and weights are fetched together first, so that no row load waits for its slot.
+constexpr int kMaxTpb = 16;    // tokens of a block
+
+template <typename T, typename O, int NV>
+__global__ void __launch_bounds__(256) expert_combine_kernel(const CombineArgs a, int tpb) {
+  extern __shared__ int32_t sm[];
+  float* wt = reinterpret_cast<float*>(sm + tpb * a.k);
+  const int64_t t0 = (int64_t)blockIdx.x * tpb;
+  const int tokens = (int)min((int64_t)tpb, a.T - t0), nv = a.width / NV, k = a.k;
+  for (int i = threadIdx.x; i < tokens * k; i += blockDim.x) {
+    const int r = a.slots[t0 * k + i];
+    sm[i] = has_row(r, a.T * k) ? r : -1;
+    wt[i] = a.weights ? a.weights[(t0 + i / k) * a.ws + i % k] : 1.f;
+  }
+  __syncthreads();
+  const T* y = static_cast<const T*>(a.y);
+  const int step = gridDim.y * blockDim.x;
+  for (int t = 0; t < tokens; ++t) {
+    for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < nv; c += step) {
+      const int64_t col = (int64_t)c * NV;
+      float acc[NV];
+      if (a.residual) {
+        Raw<O, NV> res;
+        res.load(static_cast<const O*>(a.residual) + (t0 + t) * a.rs + col);
+        res.get(acc);
+      } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) acc[i] = 0.f;
+      }
+      for (int j0 = 0; j0 < k; j0 += kBatch) {
+        const int32_t* slot = sm + t * k + j0;
+        const float* w = wt + t * k + j0;
+        Raw<T, NV> v[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+          if (j0 + j < k && slot[j] >= 0) v[j].load(y + (int64_t)slot[j] * a.ys + col);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+          if (j0 + j < k && slot[j] >= 0) {  // a pair without a row adds nothing, whatever its weight holds
+            float f[NV];
+            v[j].get(f);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) acc[i] = fmaf(w[j], f[i], acc[i]);
+          }
+      }
+      store_n<O, NV>(static_cast<O*>(a.out) + (t0 + t) * a.width + col, acc);
+    }
   }
 }
 
@@ -327,11 +400,15 @@ template <typename T, typename O>
 void combine_typed(const CombineArgs& a, bool vec, cudaStream_t stream) {
   const int nv = vec ? a.width / 8 : a.width;
   const int threads = nv >= 256 ? 256 : 128;
-  const dim3 grid((unsigned)a.T, column_parts(a.T, nv, threads, a.num_sms));
+  const unsigned parts = column_parts(a.T, nv, threads, a.num_sms);
+  int64_t tpb = a.T * parts / (8 * (int64_t)a.num_sms);  // tokens of a block, while every SM has eight blocks
+  tpb = tpb < 1 ? 1 : tpb > kMaxTpb ? kMaxTpb : tpb;
+  const dim3 grid((unsigned)((a.T + tpb - 1) / tpb), parts);
+  const size_t smem = (size_t)tpb * a.k * 8;
   if (vec)
-    expert_combine_kernel<T, O, 8><<<grid, threads, 0, stream>>>(a);
+    expert_combine_kernel<T, O, 8><<<grid, threads, smem, stream>>>(a, (int)tpb);
   else
-    expert_combine_kernel<T, O, 1><<<grid, threads, 0, stream>>>(a);
+    expert_combine_kernel<T, O, 1><<<grid, threads, smem, stream>>>(a, (int)tpb);
 }
 template <typename T, typename O>
 void combine_bwd_typed(const CombineBwdArgs& a, bool vec, cudaStream_t stream) {
@@ -343,17 +420,19 @@ void combine_bwd_typed(const CombineBwdArgs& a, bool vec, cudaStream_t stream) {
 
 }  // namespace
 
-int launch_expert_order(const void* ids, bool wide, int64_t id_stride, int64_t T, int k, int64_t base, int E,
-                        int32_t* offsets, int32_t* slots, int32_t* pairs, cudaStream_t stream) {
-  const int64_t n = T * k;
-  // one CTA up to 4096 pairs; beyond, about 4096 pairs a CTA
-  const int cluster = n <= 4096 ? 1 : n <= 8192 ? 2 : n <= 16384 ? 4 : 8;
+int launch_expert_order(const void* ids, bool wide, int64_t n, int64_t base, int E, int32_t* offsets, int32_t* slots,
+                        int32_t* pairs, cudaStream_t stream) {
+  // CTAs of the cluster: about 512 pairs each (one chunk of 32 a warp), at most 16, as long as the counts of
+  // eight warps fit shared memory.  32768 pairs, 256 experts: 7.4 us with 16 CTAs, 10.0 with 8, 19.4 with 4.
+  int cluster = 1;
+  while (cluster < 16 && (int64_t)cluster * 512 < n) cluster *= 2;
   int warps = (int)((n + 32 * cluster - 1) / (32 * cluster));
-  warps = warps < 4 ? 4 : warps > 32 ? 32 : warps;
-  const int most = (200 * 1024 / 4 - 2 * E) / E;  // shared memory: (warps + 2) counters of every expert
+  warps = warps < 4 ? 4 : warps > 16 ? 16 : warps;
+  const int most = 200 * 1024 / 4 / E - cluster;  // shared memory: (warps + CTAs) counters of every expert
+  while (cluster > 1 && 200 * 1024 / 4 / E - cluster < 8) cluster /= 2;
   warps = warps > most ? most : warps;
   if (warps < 1) return -1;
-  const size_t smem = (size_t)(warps + 2) * E * sizeof(int32_t);
+  const size_t smem = (size_t)(warps + cluster) * E * sizeof(int32_t);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(cluster);
   cfg.blockDim = dim3(warps * 32);
@@ -365,14 +444,13 @@ int launch_expert_order(const void* ids, bool wide, int64_t id_stride, int64_t T
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  if (wide) {
-    cudaFuncSetAttribute(expert_order_kernel<int64_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    return (int)cudaLaunchKernelEx(&cfg, expert_order_kernel<int64_t>, static_cast<const int64_t*>(ids), id_stride, k,
-                                   (int)n, base, E, offsets, slots, pairs);
-  }
-  cudaFuncSetAttribute(expert_order_kernel<int32_t>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  return (int)cudaLaunchKernelEx(&cfg, expert_order_kernel<int32_t>, static_cast<const int32_t*>(ids), id_stride, k,
-                                 (int)n, base, E, offsets, slots, pairs);
+  auto go = [&](auto* fn, auto* p) {
+    cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (cluster > 8) cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    return (int)cudaLaunchKernelEx(&cfg, fn, p, (int)n, base, E, offsets, slots, pairs);
+  };
+  return wide ? go(expert_order_kernel<int64_t>, static_cast<const int64_t*>(ids))
+              : go(expert_order_kernel<int32_t>, static_cast<const int32_t*>(ids));
 }
 
 void launch_expert_gather(const GatherArgs& a, cudaStream_t stream) {

@@ -264,6 +264,8 @@ struct NormMxArgs {
   void* h;            // [rows, n], optional
   uint8_t* codes;     // [rows, n]
   uint8_t* scales;    // [rows, n / 32]
+  int num_sms;
+  int* err;
 };
 void launch_add_rmsnorm_mx(const NormMxArgs& a, cudaStream_t stream);
 
@@ -283,13 +285,14 @@ struct NormBwdArgs {
   float* dxf;         // [rows, n], optional: dx before its rounding
   float* part;        // workspace [slots, n]
   float* dw;          // [n]
+  int* err;
 };
-int rmsnorm_bwd_slots(int64_t rows, int n, int num_sms);
+int rmsnorm_bwd_slots(int64_t rows, int n, bool res, int num_sms);
 void launch_rmsnorm_bwd(const NormBwdArgs& a, int slots, cudaStream_t stream);
 
 // Token rows sorted by expert and back (csrc/expert_dispatch.cu).
-int launch_expert_order(const void* ids, bool wide, int64_t id_stride, int64_t T, int k, int64_t base, int E,
-                        int32_t* offsets, int32_t* slots, int32_t* pairs, cudaStream_t stream);
+int launch_expert_order(const void* ids, bool wide, int64_t n, int64_t base, int E, int32_t* offsets, int32_t* slots,
+                        int32_t* pairs, cudaStream_t stream);
 struct GatherArgs {
   int64_t T;
   int k, E, num_sms;

@@ -2,6 +2,7 @@
 // expert_mm.cu): argument validation, output allocation, then the plain launchers.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <string>
@@ -14,6 +15,10 @@ using OptTensor = c10::optional<Tensor>;
 
 cudaStream_t stream() { return at::cuda::getCurrentCUDAStream(); }
 int sms(const Tensor& t) { return at::cuda::getDeviceProperties(t.get_device())->multiProcessorCount; }
+Tensor make(at::IntArrayRef size, const Tensor& like, torch::ScalarType type) {
+  return at::detail::empty_cuda(size, type, like.device(), c10::nullopt);
+}
+Tensor make(at::IntArrayRef size, const Tensor& like) { return make(size, like, like.scalar_type()); }
 bool is16(const Tensor& t) { return t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kFloat16; }
 bool on16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 // a row of a two-dimensional tensor that has one row may report any stride
@@ -37,6 +42,20 @@ void check_rows16(const Tensor& like, const Tensor& t, int64_t rows, int64_t n, 
   TORCH_CHECK(t.numel() == 0 || (on16(t) && row_stride(t) * t.element_size() % 16 == 0), name,
               " rows must start on 16-byte boundaries");
 }
+// t itself if its rows are contiguous and start on 16-byte boundaries, else a copy whose rows do
+Tensor rows16(const Tensor& t) {
+  if (t.dim() != 2 || t.numel() == 0 || (t.stride(1) == 1 && on16(t) && row_stride(t) * t.element_size() % 16 == 0)) return t;
+  return t.is_contiguous() ? t.clone() : t.contiguous();
+}
+OptTensor rows16(const OptTensor& t) { return t ? OptTensor(rows16(*t)) : t; }
+// t itself if its rows are contiguous, else a copy
+Tensor packed_rows(const Tensor& t) { return t.dim() != 2 || t.numel() == 0 || t.stride(1) == 1 ? t : t.contiguous(); }
+OptTensor packed_rows(const OptTensor& t) { return t ? OptTensor(packed_rows(*t)) : t; }
+void check_err(const Tensor& like, const Tensor& err) {
+  check_device(like, err, "err");
+  TORCH_CHECK(err.scalar_type() == torch::kInt32 && err.numel() >= 4, "err must be CUDA int32[4]");
+}
+
 void check_weight(const Tensor& like, const Tensor& w, int64_t n) {
   check_device(like, w, "w");
   TORCH_CHECK(w.scalar_type() == torch::kFloat32 && w.dim() == 1 && w.size(0) == n && w.is_contiguous() && on16(w),
@@ -50,10 +69,13 @@ void check_norm(const Tensor& x, const char* op) {
 }  // namespace
 
 // -> (stream, codes, scales, h or None); stream is x itself without addends or in place
-std::tuple<Tensor, Tensor, Tensor, OptTensor> add_rmsnorm_mx(const Tensor& x, const Tensor& w, double eps,
-                                                             const OptTensor& d, const OptTensor& df, bool inplace,
-                                                             bool return_h) {
-  check_norm(x, "add_rmsnorm_mx");
+std::tuple<Tensor, Tensor, Tensor, OptTensor> add_rmsnorm_mx(const Tensor& x_in, const Tensor& w, double eps,
+                                                             const OptTensor& d_in, const OptTensor& df_in, bool inplace,
+                                                             bool return_h, const Tensor& err) {
+  check_norm(x_in, "add_rmsnorm_mx");
+  check_err(x_in, err);
+  const Tensor x = inplace ? x_in : rows16(x_in);
+  const OptTensor d = rows16(d_in), df = rows16(df_in);
   const int64_t rows = x.size(0), n = x.size(1);
   check_rows16(x, x, rows, n, x.scalar_type(), "x");
   check_weight(x, w, n);
@@ -61,11 +83,11 @@ std::tuple<Tensor, Tensor, Tensor, OptTensor> add_rmsnorm_mx(const Tensor& x, co
   if (df) check_rows16(x, *df, rows, n, torch::kFloat32, "dfp32");
   const c10::cuda::CUDAGuard g(x.device());
   const bool add = d || df;
-  Tensor s = add && !inplace ? torch::empty({rows, n}, x.options()) : x;
-  Tensor codes = torch::empty({rows, n}, x.options().dtype(torch::kUInt8));
-  Tensor scales = torch::empty({rows, n / 32}, x.options().dtype(torch::kUInt8));
+  Tensor s = add && !inplace ? make({rows, n}, x) : x_in;
+  Tensor codes = make({rows, n}, x, torch::kUInt8);
+  Tensor scales = make({rows, n / 32}, x, torch::kUInt8);
   OptTensor h;
-  if (return_h) h = torch::empty({rows, n}, x.options());
+  if (return_h) h = make({rows, n}, x);
   NormMxArgs a{};
   a.rows = rows;
   a.n = (int)n;
@@ -80,27 +102,32 @@ std::tuple<Tensor, Tensor, Tensor, OptTensor> add_rmsnorm_mx(const Tensor& x, co
   if (h) a.h = h->data_ptr();
   a.codes = codes.data_ptr<uint8_t>();
   a.scales = scales.data_ptr<uint8_t>();
+  a.num_sms = sms(x);
+  a.err = err.data_ptr<int>();
   launch_add_rmsnorm_mx(a, stream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {s, codes, scales, h};
 }
 
 // -> (dx in x's type, dw fp32, dx in fp32 or None)
-std::tuple<Tensor, Tensor, OptTensor> rmsnorm_backward(const Tensor& dh, const Tensor& x, const Tensor& w, double eps,
-                                                       const OptTensor& dres, bool fp32_dx) {
-  check_norm(x, "add_rmsnorm_backward");
+std::tuple<Tensor, Tensor, OptTensor> rmsnorm_backward(const Tensor& dh_in, const Tensor& x_in, const Tensor& w,
+                                                       double eps, const OptTensor& dres_in, bool fp32_dx,
+                                                       const Tensor& err) {
+  check_norm(x_in, "add_rmsnorm_backward");
+  check_err(x_in, err);
+  const Tensor x = rows16(x_in), dh = rows16(dh_in);
+  const OptTensor dres = rows16(dres_in);
   const int64_t rows = x.size(0), n = x.size(1);
   check_rows16(x, x, rows, n, x.scalar_type(), "x");
   check_rows16(x, dh, rows, n, x.scalar_type(), "dh");
   check_weight(x, w, n);
   if (dres) check_rows16(x, *dres, rows, n, x.scalar_type(), "dres");
   const c10::cuda::CUDAGuard g(x.device());
-  const int slots = rmsnorm_bwd_slots(rows, (int)n, sms(x));
-  const auto f32 = x.options().dtype(torch::kFloat32);
-  Tensor dx = torch::empty({rows, n}, x.options()), dw = torch::empty({n}, f32);
-  Tensor part = torch::empty({slots, n}, f32);
+  const int slots = rmsnorm_bwd_slots(rows, (int)n, dres.has_value(), sms(x));
+  Tensor dx = make({rows, n}, x), dw = make({n}, x, torch::kFloat32);
+  Tensor part = make({slots, n}, x, torch::kFloat32);
   OptTensor dxf;
-  if (fp32_dx) dxf = torch::empty({rows, n}, f32);
+  if (fp32_dx) dxf = make({rows, n}, x, torch::kFloat32);
   NormBwdArgs a{};
   a.rows = rows;
   a.n = (int)n;
@@ -116,26 +143,28 @@ std::tuple<Tensor, Tensor, OptTensor> rmsnorm_backward(const Tensor& dh, const T
   if (dxf) a.dxf = dxf->data_ptr<float>();
   a.part = part.data_ptr<float>();
   a.dw = dw.data_ptr<float>();
+  a.err = err.data_ptr<int>();
   launch_rmsnorm_bwd(a, slots, stream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {dx, dw, dxf};
 }
 
 // -> (offsets [E + 1], slots [T, k], pairs [T k])
-std::tuple<Tensor, Tensor, Tensor> expert_order(const Tensor& ids, int64_t num_experts, int64_t expert_base) {
+std::tuple<Tensor, Tensor, Tensor> expert_order(const Tensor& ids_in, int64_t num_experts, int64_t expert_base) {
+  const Tensor ids = ids_in.contiguous();
   TORCH_CHECK(ids.is_cuda() && ids.dim() == 2 &&
               (ids.scalar_type() == torch::kInt32 || ids.scalar_type() == torch::kInt64),
               "expert_order: ids must be a CUDA int32 or int64 [tokens, topk] tensor");
   TORCH_CHECK(num_experts >= 1 && num_experts <= 4096, "expert_order: num_experts must be in [1, 4096]");
-  TORCH_CHECK(ids.numel() == 0 || ids.size(1) == 1 || ids.stride(1) == 1, "expert_order: a token's ids must be contiguous");
-  TORCH_CHECK(ids.numel() < (1 << 30), "expert_order: at most 2^30 pairs");
+  TORCH_CHECK(ids.numel() < (1 << 30) && ids.size(1) <= 1024, "expert_order: at most 2^30 pairs and 1024 choices");
   const c10::cuda::CUDAGuard g(ids.device());
   const int64_t T = ids.size(0), k = ids.size(1);
   const auto i32 = ids.options().dtype(torch::kInt32);
   if (T * k == 0) return {torch::zeros({num_experts + 1}, i32), torch::empty({T, k}, i32), torch::empty({0}, i32)};
-  Tensor offsets = torch::empty({num_experts + 1}, i32), slots = torch::empty({T, k}, i32), pairs = torch::empty({T * k}, i32);
-  const int rc = launch_expert_order(ids.data_ptr(), ids.scalar_type() == torch::kInt64, T == 1 ? k : ids.stride(0), T,
-                                     (int)k, expert_base, (int)num_experts, offsets.data_ptr<int32_t>(),
+  Tensor offsets = make({num_experts + 1}, ids, torch::kInt32), slots = make({T, k}, ids, torch::kInt32),
+         pairs = make({T * k}, ids, torch::kInt32);
+  const int rc = launch_expert_order(ids.data_ptr(), ids.scalar_type() == torch::kInt64, T * k, expert_base,
+                                     (int)num_experts, offsets.data_ptr<int32_t>(),
                                      slots.data_ptr<int32_t>(), pairs.data_ptr<int32_t>(), stream());
   TORCH_CHECK(rc == 0, "expert_order: launch failed (", num(rc), ")");
   C10_CUDA_KERNEL_LAUNCH_CHECK();
@@ -148,23 +177,25 @@ void check_order(const Tensor& like, const Tensor& offsets, const Tensor& slots)
   check_device(like, slots, "slots");
   TORCH_CHECK(offsets.scalar_type() == torch::kInt32 && offsets.dim() == 1 && offsets.size(0) >= 2 &&
               offsets.is_contiguous(), "offsets must be contiguous int32 [experts + 1]");
-  TORCH_CHECK(slots.scalar_type() == torch::kInt32 && slots.dim() == 2 && slots.is_contiguous(),
-              "slots must be contiguous int32 [tokens, topk]");
+  TORCH_CHECK(slots.scalar_type() == torch::kInt32 && slots.dim() == 2 && slots.is_contiguous() &&
+              slots.size(1) <= 1024, "slots must be contiguous int32 [tokens, topk], topk at most 1024");
 }
 }  // namespace
 
 // x [T, width] (and scales [T, ...], uint8) -> the same for the sorted rows
-std::tuple<Tensor, OptTensor> expert_gather(const Tensor& x, const OptTensor& scales, const Tensor& slots,
+std::tuple<Tensor, OptTensor> expert_gather(const Tensor& x_in, const OptTensor& scales_in, const Tensor& slots,
                                             const Tensor& offsets) {
+  const Tensor x = packed_rows(x_in);
+  const OptTensor scales = packed_rows(scales_in);
   TORCH_CHECK(x.is_cuda() && x.dim() == 2, "gather: x must be a CUDA [tokens, width] tensor");
   check_order(x, offsets, slots);
   const int64_t T = slots.size(0), k = slots.size(1);
   check_rows(x, x, T, x.size(1), x.scalar_type(), "x");
   if (scales) check_rows(x, *scales, T, scales->size(1), torch::kUInt8, "scales");
   const c10::cuda::CUDAGuard g(x.device());
-  Tensor out = torch::empty({T * k, x.size(1)}, x.options());
+  Tensor out = make({T * k, x.size(1)}, x);
   OptTensor sout;
-  if (scales) sout = torch::empty({T * k, scales->size(1)}, scales->options());
+  if (scales) sout = make({T * k, scales->size(1)}, *scales);
   GatherArgs a{};
   a.T = T;
   a.k = (int)k;
@@ -196,8 +227,10 @@ int row_type(const Tensor& y, const char* op) {
 bool wide(const Tensor& t) { return t.size(1) % 8 == 0 && on16(t) && row_stride(t) * t.element_size() % 16 == 0; }
 }  // namespace
 
-Tensor expert_combine(const Tensor& y, const OptTensor& weights, const OptTensor& residual, const Tensor& slots,
-                      const Tensor& offsets, bool out_f32) {
+Tensor expert_combine(const Tensor& y_in, const OptTensor& weights_in, const OptTensor& residual_in,
+                      const Tensor& slots, const Tensor& offsets, bool out_f32) {
+  const Tensor y = packed_rows(y_in);
+  const OptTensor weights = packed_rows(weights_in), residual = packed_rows(residual_in);
   const int type = row_type(y, "combine");
   check_order(y, offsets, slots);
   const int64_t T = slots.size(0), k = slots.size(1), width = y.size(1);
@@ -206,7 +239,7 @@ Tensor expert_combine(const Tensor& y, const OptTensor& weights, const OptTensor
   if (weights) check_rows(y, *weights, T, k, torch::kFloat32, "weights");
   if (residual) check_rows(y, *residual, T, width, out_type, "residual");
   const c10::cuda::CUDAGuard g(y.device());
-  Tensor out = torch::empty({T, width}, y.options().dtype(out_type));
+  Tensor out = make({T, width}, y, out_type);
   CombineArgs a{};
   a.T = T;
   a.k = (int)k;
@@ -224,9 +257,10 @@ Tensor expert_combine(const Tensor& y, const OptTensor& weights, const OptTensor
 }
 
 // -> (dy or None, dweights or None)
-std::tuple<OptTensor, OptTensor> expert_combine_backward(const Tensor& dout, const Tensor& y, const Tensor& weights,
-                                                         const Tensor& slots, const Tensor& offsets, bool need_dy,
-                                                         bool need_dw) {
+std::tuple<OptTensor, OptTensor> expert_combine_backward(const Tensor& dout_in, const Tensor& y_in,
+                                                         const Tensor& weights_in, const Tensor& slots,
+                                                         const Tensor& offsets, bool need_dy, bool need_dw) {
+  const Tensor dout = packed_rows(dout_in), y = packed_rows(y_in), weights = packed_rows(weights_in);
   const int type = row_type(y, "combine_backward");
   check_order(y, offsets, slots);
   const int64_t T = slots.size(0), k = slots.size(1), width = y.size(1);
@@ -237,8 +271,8 @@ std::tuple<OptTensor, OptTensor> expert_combine_backward(const Tensor& dout, con
   check_rows(y, dout, T, width, dout.scalar_type(), "dout");
   const c10::cuda::CUDAGuard g(y.device());
   OptTensor dy, dw;
-  if (need_dy) dy = torch::empty({T * k, width}, y.options());
-  if (need_dw) dw = torch::empty({T, k}, weights.options());
+  if (need_dy) dy = make({T * k, width}, y);
+  if (need_dw) dw = make({T, k}, weights);
   CombineBwdArgs a{};
   a.T = T;
   a.k = (int)k;
@@ -270,8 +304,7 @@ void check_mm(const Tensor& w, const Tensor& offsets, const Tensor& err, const c
   check_device(w, offsets, "offsets");
   TORCH_CHECK(offsets.scalar_type() == torch::kInt32 && offsets.dim() == 1 && offsets.size(0) == w.size(0) + 1 &&
               offsets.is_contiguous(), op, ": offsets must be contiguous int32 [experts + 1]");
-  check_device(w, err, "err");
-  TORCH_CHECK(err.scalar_type() == torch::kInt32 && err.numel() >= 4, "err must be CUDA int32[4]");
+  check_err(w, err);
 }
 ExpertMmCall mm_call(const Tensor& w, const Tensor& offsets, const Tensor& err, int64_t P) {
   TORCH_CHECK(P < (1 << 30), "at most 2^30 rows");
@@ -295,17 +328,18 @@ void run_mm(int mode, const ExpertMmCall& c) {
 }  // namespace
 
 // -> (y, the products z or None); gated: y = silu(z[:, :n / 2]) z[:, n / 2:]
-std::tuple<Tensor, OptTensor> expert_mm(const Tensor& x, const Tensor& w, const Tensor& offsets, bool gated,
+std::tuple<Tensor, OptTensor> expert_mm(const Tensor& x_in, const Tensor& w, const Tensor& offsets, bool gated,
                                         bool save_pre, const Tensor& err) {
   check_mm(w, offsets, err, "expert_linear");
+  const Tensor x = rows16(x_in);
   const int64_t P = x.size(0), N = w.size(1), K = w.size(2);
   check_rows16(w, x, P, K, w.scalar_type(), "x");
   TORCH_CHECK(!gated || N % 16 == 0, "expert_linear: a gated product needs n a multiple of 16");
   TORCH_CHECK(gated || !save_pre, "expert_linear: only a gated product keeps its operands");
   const c10::cuda::CUDAGuard g(w.device());
-  Tensor y = torch::empty({P, gated ? N / 2 : N}, x.options());
+  Tensor y = make({P, gated ? N / 2 : N}, x);
   OptTensor pre;
-  if (save_pre) pre = torch::empty({P, N}, x.options());
+  if (save_pre) pre = make({P, N}, x);
   if (P > 0) {
     ExpertMmCall c = mm_call(w, offsets, err, P);
     c.x = x.data_ptr();
@@ -319,17 +353,18 @@ std::tuple<Tensor, OptTensor> expert_mm(const Tensor& x, const Tensor& w, const 
 }
 
 // -> (dx or None, dw or None)
-std::tuple<OptTensor, OptTensor> expert_mm_backward(const Tensor& dz, const Tensor& x, const Tensor& w,
+std::tuple<OptTensor, OptTensor> expert_mm_backward(const Tensor& dz_in, const Tensor& x_in, const Tensor& w,
                                                     const Tensor& offsets, bool need_dx, bool need_dw,
                                                     const Tensor& err) {
   check_mm(w, offsets, err, "expert_linear_backward");
+  const Tensor x = rows16(x_in), dz = rows16(dz_in);
   const int64_t P = x.size(0), N = w.size(1), K = w.size(2);
   check_rows16(w, x, P, K, w.scalar_type(), "x");
   check_rows16(w, dz, P, N, w.scalar_type(), "dy");
   const c10::cuda::CUDAGuard g(w.device());
   OptTensor dx, dw;
-  if (need_dx) dx = torch::empty({P, K}, x.options());
-  if (need_dw) dw = P > 0 ? torch::empty_like(w) : torch::zeros_like(w);
+  if (need_dx) dx = make({P, K}, x);
+  if (need_dw) dw = P > 0 ? make(w.sizes(), w) : torch::zeros_like(w);
   if (P > 0) {
     ExpertMmCall c = mm_call(w, offsets, err, P);
     c.x = x.data_ptr();
@@ -342,7 +377,8 @@ std::tuple<OptTensor, OptTensor> expert_mm_backward(const Tensor& dz, const Tens
   return {dx, dw};
 }
 
-Tensor swiglu_backward(const Tensor& da, const Tensor& pre, const Tensor& offsets) {
+Tensor swiglu_backward(const Tensor& da_in, const Tensor& pre_in, const Tensor& offsets) {
+  const Tensor da = rows16(da_in), pre = rows16(pre_in);
   TORCH_CHECK(pre.is_cuda() && pre.dim() == 2 && is16(pre) && pre.size(1) >= 16 && pre.size(1) % 16 == 0,
               "swiglu_backward: pre must be a CUDA BF16 or FP16 [rows, n] tensor, n a multiple of 16");
   const int64_t P = pre.size(0), N = pre.size(1);
@@ -352,7 +388,7 @@ Tensor swiglu_backward(const Tensor& da, const Tensor& pre, const Tensor& offset
   TORCH_CHECK(offsets.scalar_type() == torch::kInt32 && offsets.dim() == 1 && offsets.size(0) >= 2 &&
               offsets.is_contiguous(), "swiglu_backward: offsets must be contiguous int32 [experts + 1]");
   const c10::cuda::CUDAGuard g(pre.device());
-  Tensor dz = torch::empty({P, N}, pre.options());
+  Tensor dz = make({P, N}, pre);
   launch_swiglu_bwd(da.data_ptr(), row_stride(da), pre.data_ptr(), row_stride(pre), dz.data_ptr(), P, (int)(N / 2),
                     offsets.data_ptr<int32_t>(), (int)offsets.size(0) - 1, pre.scalar_type() == torch::kFloat16,
                     sms(pre), stream());
@@ -360,14 +396,143 @@ Tensor swiglu_backward(const Tensor& da, const Tensor& pre, const Tensor& offset
   return dz;
 }
 
+// ----------------------------------------------------------------------------- autograd
+// The differentiable entry points: where a gradient is recorded they run as autograd nodes, else directly.
+namespace {
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
+
+bool wanted(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t && t->defined() && t->requires_grad()) return true;
+  return false;
+}
+const Tensor* at_or_null(const OptTensor& t) { return t ? &*t : nullptr; }
+void check_once() { TORCH_CHECK(!at::GradMode::is_enabled(), "the expert block operators have no second derivative"); }
+OptTensor some(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+struct AddRmsNormMx : Function<AddRmsNormMx> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& d,
+                               const OptTensor& df, double eps, bool return_h, const Tensor& err) {
+    auto [s, codes, scales, h] = add_rmsnorm_mx(x, w, eps, d, df, false, return_h, err);
+    ctx->save_for_backward({s, w, err});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["d"] = d.has_value();
+    ctx->saved_data["df"] = df.has_value();
+    ctx->mark_non_differentiable({codes, scales});
+    ctx->set_materialize_grads(false);
+    variable_list out{s, codes, scales};
+    if (h) out.push_back(*h);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_once();
+    const auto saved = ctx->get_saved_variables();
+    const bool has_d = ctx->saved_data["d"].toBool(), has_f = ctx->saved_data["df"].toBool();
+    const Tensor ds = g[0], dh = g.size() > 3 ? g[3] : Tensor();
+    Tensor dx = ds, dw, dxf;
+    if (dh.defined()) {
+      auto [a, b, c] = rmsnorm_backward(dh, saved[0], saved[1], ctx->saved_data["eps"].toDouble(), some(ds), has_f, saved[2]);
+      dx = a;
+      dw = b;
+      if (c) dxf = *c;
+    } else if (has_f && ds.defined()) {
+      dxf = ds.to(torch::kFloat32);  // only the stream was used
+    }
+    return {dx, dw, has_d ? dx : Tensor(), dxf, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+struct Gather : Function<Gather> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& slots, const Tensor& offsets) {
+    ctx->save_for_backward({slots, offsets});
+    return std::get<0>(expert_gather(x, c10::nullopt, slots, offsets));
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_once();
+    const auto saved = ctx->get_saved_variables();
+    return {expert_combine(g[0], c10::nullopt, c10::nullopt, saved[0], saved[1], false), Tensor(), Tensor()};
+  }
+};
+
+struct Combine : Function<Combine> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& y, const OptTensor& weights, const OptTensor& residual,
+                        const Tensor& slots, const Tensor& offsets, bool out_f32) {
+    ctx->save_for_backward({y, weights ? *weights : Tensor(), slots, offsets});
+    ctx->saved_data["res"] = residual.has_value();
+    return expert_combine(y, weights, residual, slots, offsets, out_f32);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_once();
+    const auto saved = ctx->get_saved_variables();
+    const Tensor& y = saved[0];
+    const Tensor& weights = saved[1];
+    const bool need_dy = ctx->needs_input_grad(0), need_dw = weights.defined() && ctx->needs_input_grad(1);
+    Tensor dy, dw;
+    if (!weights.defined()) {
+      if (need_dy) dy = std::get<0>(expert_gather(g[0], c10::nullopt, saved[2], saved[3])).to(y.scalar_type());
+    } else {
+      auto [a, b] = expert_combine_backward(g[0], y, weights, saved[2], saved[3], need_dy, need_dw);
+      if (a) dy = *a;
+      if (b) dw = *b;
+    }
+    return {dy, dw, ctx->saved_data["res"].toBool() ? g[0] : Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+struct ExpertLinear : Function<ExpertLinear> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& offsets, bool gated,
+                        const Tensor& err) {
+    auto [y, pre] = expert_mm(x, w, offsets, gated, gated, err);
+    ctx->save_for_backward({x, w, offsets, pre ? *pre : Tensor(), err});
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_once();
+    const auto saved = ctx->get_saved_variables();
+    const Tensor dz = saved[3].defined() ? swiglu_backward(g[0], saved[3], saved[2]) : g[0];
+    auto [dx, dw] = expert_mm_backward(dz, saved[0], saved[1], saved[2], ctx->needs_input_grad(0),
+                                       ctx->needs_input_grad(1), saved[4]);
+    return {dx ? *dx : Tensor(), dw ? *dw : Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+}  // namespace
+
+std::tuple<Tensor, Tensor, Tensor, OptTensor> add_rmsnorm_mx_op(const Tensor& x, const Tensor& w, double eps,
+                                                                const OptTensor& d, const OptTensor& df, bool inplace,
+                                                                bool return_h, const Tensor& err) {
+  if (!wanted({&x, &w, at_or_null(d), at_or_null(df)})) return add_rmsnorm_mx(x, w, eps, d, df, inplace, return_h, err);
+  TORCH_CHECK(!inplace, "add_rmsnorm_mx: inplace is not available where a gradient is recorded");
+  variable_list o = AddRmsNormMx::apply(x, w, d, df, eps, return_h, err);
+  return {o[0], o[1], o[2], return_h ? OptTensor(o[3]) : OptTensor()};
+}
+Tensor gather_op(const Tensor& x, const Tensor& slots, const Tensor& offsets) {
+  if (!wanted({&x})) return std::get<0>(expert_gather(x, c10::nullopt, slots, offsets));
+  return Gather::apply(x, slots, offsets);
+}
+Tensor combine_op(const Tensor& y, const OptTensor& weights, const OptTensor& residual, const Tensor& slots,
+                  const Tensor& offsets, bool out_f32) {
+  if (!wanted({&y, at_or_null(weights), at_or_null(residual)}))
+    return expert_combine(y, weights, residual, slots, offsets, out_f32);
+  return Combine::apply(y, weights, residual, slots, offsets, out_f32);
+}
+Tensor expert_linear_op(const Tensor& x, const Tensor& w, const Tensor& offsets, bool gated, const Tensor& err) {
+  if (!wanted({&x, &w})) return std::get<0>(expert_mm(x, w, offsets, gated, false, err));
+  return ExpertLinear::apply(x, w, offsets, gated, err);
+}
+
 void bind_block_ops(pybind11::module_& m) {
-  m.def("add_rmsnorm_mx", &add_rmsnorm_mx, "residual add + RMSNorm -> MXFP8 rows");
-  m.def("rmsnorm_backward", &rmsnorm_backward, "gradient of residual add + RMSNorm");
-  m.def("expert_order", &expert_order, "stable sort of (token, choice) pairs by expert");
-  m.def("expert_gather", &expert_gather, "token rows -> rows sorted by expert");
-  m.def("expert_combine", &expert_combine, "rows sorted by expert -> weighted sums per token");
-  m.def("expert_combine_backward", &expert_combine_backward, "gradients of expert_combine");
-  m.def("expert_mm", &expert_mm, "every expert's matrix product (tcgen05), optionally gated");
-  m.def("expert_mm_backward", &expert_mm_backward, "gradients of expert_mm (tcgen05)");
-  m.def("swiglu_backward", &swiglu_backward, "gradient of silu(gate) * up over sorted rows");
+  const auto unlocked = pybind11::call_guard<pybind11::gil_scoped_release>();
+  m.def("add_rmsnorm_mx", &add_rmsnorm_mx_op, "residual add + RMSNorm -> MXFP8 rows", unlocked);
+  m.def("rmsnorm_backward", &rmsnorm_backward, "gradient of residual add + RMSNorm", unlocked);
+  m.def("expert_order", &expert_order, "stable sort of (token, choice) pairs by expert", unlocked);
+  m.def("expert_gather", &gather_op, "token rows -> rows sorted by expert", unlocked);
+  m.def("expert_gather_mx", &expert_gather, "MXFP8 token rows -> rows sorted by expert", unlocked);
+  m.def("expert_combine", &combine_op, "rows sorted by expert -> weighted sums per token", unlocked);
+  m.def("expert_combine_backward", &expert_combine_backward, "gradients of expert_combine", unlocked);
+  m.def("expert_linear", &expert_linear_op, "every expert's matrix product (tcgen05), optionally gated", unlocked);
+  m.def("expert_linear_backward", &expert_mm_backward, "gradients of the ungated expert_linear (tcgen05)", unlocked);
+  m.def("swiglu_backward", &swiglu_backward, "gradient of silu(gate) * up over sorted rows", unlocked);
 }

@@ -37,8 +37,6 @@ def expert_order(ids: torch.Tensor, num_experts: int, expert_base: int = 0) -> E
     if ids.dim() != 2 or ids.dtype not in (torch.int32, torch.int64):
         raise ValueError("ids must be an int32 or int64 [tokens, topk] tensor")
     if ids.is_cuda:
-        if ids.shape[1] > 1 and ids.stride(1) != 1:
-            ids = ids.contiguous()
         return ExpertOrder(*ext().expert_order(ids, num_experts, expert_base))
     flat = ids.reshape(-1).long() - expert_base
     key = torch.where((flat >= 0) & (flat < num_experts), flat, num_experts)
@@ -53,19 +51,12 @@ def expert_order(ids: torch.Tensor, num_experts: int, expert_base: int = 0) -> E
     return ExpertOrder(offsets.int(), slots.int().view(ids.shape), pairs.int())
 
 
-def _row_contiguous(t: torch.Tensor | None) -> torch.Tensor | None:
-    return t if t is None or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
-
-
 def _check_tokens(x: torch.Tensor, order: ExpertOrder, name: str) -> None:
     if x.dim() != 2 or x.shape[0] != order.slots.shape[0]:
         raise ValueError(f"{name} must be [{order.slots.shape[0]}, width]: one row per token of the order")
 
 
 def _gather(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
-    _check_tokens(x, order, "x")
-    if x.is_cuda:
-        return ext().expert_gather(_row_contiguous(x), None, order.slots, order.offsets)[0]
     token = order.pairs.clamp_min(0).long() // max(1, order.slots.shape[1])
     zero = torch.zeros((), dtype=x.dtype)
     return torch.where((order.pairs >= 0)[:, None], x[token], zero)
@@ -78,19 +69,16 @@ def gather_mx(codes: torch.Tensor, scales: torch.Tensor, order: ExpertOrder) -> 
     if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
         raise ValueError("codes and scales must be uint8")
     if codes.is_cuda:
-        return ext().expert_gather(_row_contiguous(codes), _row_contiguous(scales), order.slots, order.offsets)
+        return ext().expert_gather_mx(codes, scales, order.slots, order.offsets)
     return _gather(codes, order), _gather(scales, order)
 
 
 def gather_backward(drows: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     """Gradient of `gather`: dx[t] = sum over the token's rows of drows (fp32 sum, one rounding)."""
-    return _combine(drows, order, None, None, drows.dtype)
+    return combine(drows, order)
 
 
 def _combine(y, order, weights, residual, out_dtype):
-    if y.is_cuda:
-        return ext().expert_combine(_row_contiguous(y), _row_contiguous(weights), _row_contiguous(residual), order.slots,
-                                    order.offsets, out_dtype == torch.float32)
     here = order.slots >= 0
     rows = y[order.slots.clamp_min(0).long()].float() if y.shape[0] else y.new_zeros((*order.slots.shape, y.shape[1])).float()
     w = torch.where(here, weights if weights is not None else torch.ones(()), 0.0)
@@ -105,8 +93,7 @@ def combine_backward(dout: torch.Tensor, y: torch.Tensor, order: ExpertOrder, we
     """Gradients of `combine`: dy[row of (t, j)] = w[t, j] dout[t] (rows of no pair: 0) and
     dweights[t, j] = <dout[t], y[row]> in fp32 (0 for a pair without a row); each None if not needed."""
     if y.is_cuda:
-        return ext().expert_combine_backward(_row_contiguous(dout), _row_contiguous(y), _row_contiguous(weights),
-                                             order.slots, order.offsets, need_dy, need_dweights)
+        return ext().expert_combine_backward(dout, y, weights, order.slots, order.offsets, need_dy, need_dweights)
     here, at, g = order.slots >= 0, order.slots.clamp_min(0).long(), dout.float()
     dy = dw = None
     if need_dy:
@@ -118,7 +105,7 @@ def combine_backward(dout: torch.Tensor, y: torch.Tensor, order: ExpertOrder, we
     return dy, dw
 
 
-class _Gather(torch.autograd.Function):
+class _Gather(torch.autograd.Function):  # CPU tensors; the extension has its own nodes
     @staticmethod
     def forward(ctx, x, *order):
         ctx.order = ExpertOrder(*order)
@@ -154,6 +141,9 @@ def gather(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     """Rows [T k, H]: row r holds its pair's token row x[pairs[r] // k]; rows of no pair are zero.
 
     x [T, H] of any type, rows contiguous (any stride between them).  Differentiable."""
+    _check_tokens(x, order, "x")
+    if x.is_cuda:
+        return ext().expert_gather(x, order.slots, order.offsets)
     if torch.is_grad_enabled() and x.requires_grad:
         return _Gather.apply(x, *order)
     return _gather(x, order)
@@ -175,6 +165,8 @@ def combine(y: torch.Tensor, order: ExpertOrder, weights: torch.Tensor | None = 
         raise ValueError(f"weights must be fp32 {list(order.slots.shape)}")
     if residual is not None and (residual.shape != (order.slots.shape[0], y.shape[1]) or residual.dtype != out_dtype):
         raise ValueError("residual must be [tokens, width] of the output's type")
+    if y.is_cuda:
+        return ext().expert_combine(y, weights, residual, order.slots, order.offsets, out_dtype == torch.float32)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (y, weights, residual)):
         return _Combine.apply(y, weights, residual, out_dtype, *order)
     return _combine(y, order, weights, residual, out_dtype)

@@ -6,7 +6,7 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from ..formats import abi, codec
-from ._ext import ext
+from ._ext import error_word, ext
 
 
 def add_rmsnorm(x: torch.Tensor, w: torch.Tensor, eps: float, d: torch.Tensor | None = None,
@@ -126,18 +126,7 @@ def _check_norm(x: torch.Tensor, w: torch.Tensor) -> None:
         raise ValueError("w must be fp32 [n]")
 
 
-def _rows16(t: torch.Tensor | None) -> torch.Tensor | None:
-    """`t` itself if its rows are contiguous and start on 16-byte boundaries, else a contiguous copy."""
-    if t is None or (t.stride(1) == 1 and t.stride(0) * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0):
-        return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
-
-
 def _add_rmsnorm_mx(x, w, eps, d, dfp32, inplace, return_h):
-    if x.is_cuda:
-        xr = x if inplace else _rows16(x)
-        s, codes, scales, h = ext().add_rmsnorm_mx(xr, w, float(eps), _rows16(d), _rows16(dfp32), inplace, return_h)
-        return (x if d is None and dfp32 is None else s), codes, scales, h
     _check_norm(x, w)
     s = x
     if d is not None or dfp32 is not None:
@@ -157,7 +146,7 @@ def add_rmsnorm_backward(dh: torch.Tensor, x: torch.Tensor, w: torch.Tensor, eps
     Returns (dx, dw) - dx in x's type is also the gradient of the addend d, dw is fp32 and does not depend on
     timing (fixed summation order) - or (dx, dw, fp32 dx) with `fp32_dx`, the gradient of the fp32 addend."""
     if x.is_cuda:
-        dx, dw, dxf = ext().rmsnorm_backward(_rows16(dh), _rows16(x), w, float(eps), _rows16(dres), fp32_dx)
+        dx, dw, dxf = ext().rmsnorm_backward(dh, x, w, eps, dres, fp32_dx, error_word(x.device))
         return (dx, dw, dxf) if fp32_dx else (dx, dw)
     _check_norm(x, w)
     n, r = _norm_oracle(x.float(), w, eps)
@@ -169,7 +158,7 @@ def add_rmsnorm_backward(dh: torch.Tensor, x: torch.Tensor, w: torch.Tensor, eps
     return (dxf.to(x.dtype), dw, dxf) if fp32_dx else (dxf.to(x.dtype), dw)
 
 
-class _AddRmsNormMx(torch.autograd.Function):
+class _AddRmsNormMx(torch.autograd.Function):  # CPU tensors; the extension has its own node
     @staticmethod
     def forward(ctx, x, w, d, dfp32, eps, return_h):
         s, codes, scales, h = _add_rmsnorm_mx(x, w, eps, d, dfp32, False, return_h)
@@ -208,8 +197,12 @@ def add_rmsnorm_mx(x: torch.Tensor, w: torch.Tensor, eps: float, d: torch.Tensor
 
     Differentiable in x, w, d and dfp32 through x_new and h; the codes carry no gradient (a trainer that feeds
     them to its products uses h's gradient for them)."""
+    if x.is_cuda and not inplace:
+        return ext().add_rmsnorm_mx(x, w, eps, d, dfp32, False, return_h, error_word(x.device))
     wanted = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, d, dfp32))
     if not wanted:
+        if x.is_cuda:
+            return ext().add_rmsnorm_mx(x, w, eps, d, dfp32, True, return_h, error_word(x.device))
         return _add_rmsnorm_mx(x, w, eps, d, dfp32, inplace, return_h)
     if inplace:
         raise ValueError("inplace is not available where a gradient is recorded")

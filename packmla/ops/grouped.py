@@ -11,7 +11,6 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ._ext import error_word, ext
-from .fused import _rows16
 
 ACTIVATIONS = (None, "swiglu")
 
@@ -39,8 +38,6 @@ def _silu_grad(z: torch.Tensor, da: torch.Tensor) -> torch.Tensor:
 
 
 def _linear(x, w, offsets, gated: bool, save_pre: bool):
-    if w.is_cuda:
-        return ext().expert_mm(_rows16(x), w, offsets, gated, save_pre, error_word(w.device))
     z = torch.zeros(x.shape[0], w.shape[1], dtype=torch.float32)
     for e, (a, b) in enumerate(_spans(offsets, x.shape[0])):
         z[a:b] = x[a:b].float() @ w[e].float().T
@@ -57,7 +54,7 @@ def expert_linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, o
     _check(x, w, offsets, w.shape[2], "x")
     _check(dy, w, offsets, w.shape[1], "dy")
     if w.is_cuda:
-        return ext().expert_mm_backward(_rows16(dy), _rows16(x), w, offsets, need_dx, need_dw, error_word(w.device))
+        return ext().expert_linear_backward(dy, x, w, offsets, need_dx, need_dw, error_word(w.device))
     dx = torch.zeros(x.shape, dtype=torch.float32) if need_dx else None
     dw = torch.zeros(w.shape, dtype=torch.float32) if need_dw else None
     for e, (a, b) in enumerate(_spans(offsets, x.shape[0])):
@@ -76,13 +73,13 @@ def swiglu_backward(dy: torch.Tensor, pre: torch.Tensor, offsets: torch.Tensor) 
     if dy.shape != (pre.shape[0], pre.shape[1] // 2) or dy.dtype != pre.dtype:
         raise ValueError("dy must be [rows, n / 2] of pre's type")
     if pre.is_cuda:
-        return ext().swiglu_backward(_rows16(dy), _rows16(pre), offsets)
+        return ext().swiglu_backward(dy, pre, offsets)
     dz = _silu_grad(pre, dy)
     dz[_spans(offsets, pre.shape[0])[-1][1]:] = 0
     return dz.to(pre.dtype)
 
 
-class _ExpertLinear(torch.autograd.Function):
+class _ExpertLinear(torch.autograd.Function):  # CPU tensors; the extension has its own node
     @staticmethod
     def forward(ctx, x, w, offsets, gated):
         y, pre = _linear(x, w, offsets, gated, gated)
@@ -111,6 +108,8 @@ def expert_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, activ
     gated = activation == "swiglu"
     if gated and w.shape[1] % 16:
         raise ValueError("a gated product needs n a multiple of 16")
+    if w.is_cuda:
+        return ext().expert_linear(x, w, offsets, gated, error_word(w.device))
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         return _ExpertLinear.apply(x, w, offsets, gated)
     return _linear(x, w, offsets, gated, False)[0]
