@@ -7,15 +7,6 @@
 //
 // Expert e owns rows offsets[e] .. offsets[e + 1]; the offsets are read on the device, so no call waits for
 // the host.  Rows past offsets[E] give zero rows (kForward, kGradX) and are not read (kGradW).
-//
-// Tile: 128 x 256 outputs, 64 of the reduced dimension per stage, both operands by TMA with the 128-byte
-// swizzle.  Rows (x, dz) are the M = 128 operand of kForward and kGradX: an expert's last tile reads into
-// the next expert's rows, which only fills accumulator rows that nobody stores.  kGradX reads W, and kGradW
-// reads both operands, along their other dimension through MN-major descriptors, so nothing is transposed in
-// memory; kGradW reduces over rows, so the rows past the expert's last one in its last stage are zeroed in
-// shared memory before the MMA.  One persistent CTA per SM: a TMA warp, an MMA warp and four epilogue warps,
-// the accumulator double-buffered in TMEM (2 x 256 columns), so that a tile's epilogue overlaps the next
-// tile's products.
 #include <cuda.h>
 
 #include "launchers.h"
@@ -24,347 +15,445 @@
 
 namespace {
 
-constexpr int kThreads = 192;      // warp 0 TMA producer, warp 1 MMA issuer, warps 2-5 epilogue
-constexpr int kTileM = 128, kTileN = 256, kTileK = 64;
-constexpr uint32_t kBBytes = kTileN * kTileK * 2;
-constexpr uint32_t kChunk = 64 * 128;  // MN-major operands: 64 reduced rows x 64 columns (128 B)
-constexpr int kEpiWarpBytes = 32 * 128;  // staging of one epilogue warp: 32 rows x 64 outputs
-constexpr int kBand = 8;           // row tiles that walk the column tiles together (L2 reuse of both operands)
+constexpr int kTileK = 64;         // of the reduced dimension per stage: 128 bytes, one swizzle row
 constexpr int kMaxStages = 8;
 enum Mode { kForward = 0, kGradX = 1, kGradW = 2 };
 
-// AM: rows of the A operand that a stage loads (the MMA always takes 128; rows past AM read whatever the
-// stage holds and fill accumulator rows that nobody stores).
-template <int AM>
-struct Cfg {
-  static constexpr uint32_t kABytes = AM * kTileK * 2;
-  static constexpr uint32_t kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = AM == 128 ? 4 : 5;
-  static constexpr uint32_t kEpiOff = kStages * kStageBytes;
-  static constexpr uint32_t kBarOff = kEpiOff + 4 * kEpiWarpBytes;
-  static constexpr uint32_t kFixed = kBarOff + 256 + 1024;  // barriers, alignment; then the tile table
-  static_assert(kABytes % 1024 == 0 && 128 * kTileK * 2 <= kStageBytes && kStages <= kMaxStages, "stage layout");
-};
+__device__ __forceinline__ float silu(float g) { return g / (1.f + __expf(-g)); }
 
-struct Tile {
-  int e, m, n;      // expert, row tile and column tile inside it
-  int row0, rows;   // kForward / kGradX: first row and rows of the tile; kGradW: the expert's
-  int nk;           // stages (0: the tile is zero)
-};
-
-// Walks this CTA's tiles in order; every role of the CTA keeps its own walker.
-template <int MODE, int AM>
-struct Walker {
-  const ExpertMmArgs& a;
-  const int32_t* start;  // shared: first tile of each expert, [E + 2] (expert E: the rows past the last one)
-  const int32_t* off;    // shared: offsets [E + 1]
-  int tn, tm_w, e, t;
-  __device__ Walker(const ExpertMmArgs& args, const int32_t* s, const int32_t* o) : a(args), start(s), off(o) {
-    e = 0;
-    t = (int)blockIdx.x - (int)gridDim.x;
-    tn = a.tiles_n;
-    tm_w = a.tiles_m;
-  }
-  __device__ bool next(Tile& k) {
-    t += gridDim.x;
-    const int E = a.E;
-    if (t >= start[MODE == kGradW ? E : E + 1]) return false;
-    while (t >= start[e + 1]) ++e;
-    const int rel = t - start[e];
-    int tm;
-    k.e = e;
-    if (MODE == kGradW) {
-      tm = tm_w;
-      k.row0 = off[e];
-      k.rows = off[e + 1] - off[e];
-      k.nk = (k.rows + kTileK - 1) / kTileK;
-    } else {
-      const int first = off[e], last = e < E ? off[e + 1] : a.P;
-      tm = (last - first + AM - 1) / AM;
-      k.row0 = first;
-      k.rows = last - first;
-      k.nk = e < E ? a.nk : 0;
+// off[0 .. E]: offsets clamped to 0 = off[0] <= off[e] <= off[e + 1] <= P (a wrong table must not reach memory);
+// start[0 .. E + 1]: first tile of each expert, for tiles(rows of e, e) tiles each; "expert" E is the rows past
+// the last one.  Called by one warp.
+template <typename Tiles>
+__device__ __forceinline__ void tile_table(const ExpertMmArgs& a, int32_t* off, int32_t* start, int lane, Tiles tiles) {
+  int carry_off = 0, carry_t = 0;
+  for (int e0 = 0; e0 <= a.E; e0 += 32) {
+    const int e = e0 + lane;
+    int o = e > 0 && e <= a.E ? min(max(a.offsets[e], 0), a.P) : 0;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, o, s);
+      if (lane >= s) o = max(o, u);
     }
-    const int band = rel / (kBand * tn), in = rel - band * kBand * tn;
-    const int h = min(kBand, tm - band * kBand);
-    k.n = in / h;
-    k.m = band * kBand + in - k.n * h;
-    if (MODE != kGradW) {
-      k.row0 += k.m * AM;
-      k.rows = min(AM, k.rows - k.m * AM);
+    o = max(o, carry_off);
+    if (e <= a.E) off[e] = o;
+    carry_off = __shfl_sync(0xffffffffu, o, 31);
+  }
+  __syncwarp();
+  for (int e0 = 0; e0 <= a.E; e0 += 32) {
+    const int e = e0 + lane;
+    int inc = e <= a.E ? tiles((e < a.E ? off[e + 1] : a.P) - off[e], e) : 0;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, inc, s);
+      if (lane >= s) inc += u;
+    }
+    if (e <= a.E) start[e + 1] = carry_t + inc;
+    carry_t += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  if (lane == 0) start[0] = 0;
+}
+
+// ----------------------------------------------------------------------------- CTA pairs
+// A pair (a cluster of two CTAs) computes D [256 x N], N <= 256: CTA r holds rows 128 r .. of A and of D, and
+// half of B's N rows, so that each operand byte crosses from L2 to shared memory once per pair.  That crossing
+// is what bounds a single-CTA kernel: 128 x 256 tiles take 48 KB per 512 tensor cycles, 96 bytes a cycle of an
+// SM, and ran at 76 % of the tensor pipe; 256 x 256 pairs take 64 and run at 94 %.  The accumulator is
+// double-buffered in TMEM, so a tile's epilogue overlaps the next tile's products.  With few rows an expert (a
+// decode step) the weights' stream from HBM is the bound: six stages of up to 32 KB in flight per SM.
+//
+//   kForward, kGradX: A is the weight (256 output features), B the rows (tokens): D is y^T.  An expert's rows
+//     are cut into tiles of at most 256, and N is the tile's rows rounded up to 32 (the MMA's step), so a
+//     ragged expert costs its rows and not a multiple of a fixed tile.  The epilogue turns D through shared
+//     memory.  Gated: A takes gate and up rows by turns, 8 and 8, so that a feature's two products lie 8 TMEM
+//     lanes apart and meet by one exchange within the warp.
+//   kGradW: A is dz^T (256 of n), B x^T (256 of k), both MN-major, reduced over the expert's rows.  The last
+//     stage reads into the next expert's rows, and 0 x NaN is NaN: each CTA zeroes those rows of both its
+//     operands in shared memory before the MMA.
+//   kGradX reads W along its other dimension by an MN-major descriptor: nothing is transposed in memory.
+constexpr int kPairThreads = 320;  // warp 0 TMA producer, 1 MMA issuer (leader) / tail rows, 2-9 epilogue
+constexpr int kEpiWarps = 8;
+constexpr uint32_t kEpiWarpBytes = 32 * 64;  // staging of an epilogue warp: 32 rows x 32 columns
+constexpr uint32_t kHalf = 128 * 128;    // 128 rows x 64 elements: one CTA's A rows, or its half of B
+constexpr uint32_t kChunk = 64 * 128;    // MN-major operands: 64 reduced rows x 64 columns
+constexpr int kBand = 8;                 // row tiles that walk the feature tiles together (L2 reuse of both)
+
+struct Pair {
+  static constexpr uint32_t kABytes = kHalf;
+  static constexpr uint32_t kStageBytes = kABytes + kHalf;
+  static constexpr int kStages = 6;
+  static constexpr uint32_t kEpiOff = kStages * kStageBytes;
+  static constexpr uint32_t kBarOff = kEpiOff + kEpiWarps * kEpiWarpBytes;
+  static constexpr uint32_t kTableOff = kBarOff + 512;
+  static constexpr uint32_t kFixed = kTableOff + 1024;  // and alignment; then the tile table
+};
+
+struct PairTile {
+  int e, m, n;     // expert; feature tile (n of dW); row tile (k of dW)
+  int row0, rows;  // kForward / kGradX: the tile's rows; kGradW: the expert's
+  int cols;        // B rows of the MMA: a multiple of 32
+  int nk;          // stages (0: the tile is zero)
+};
+
+template <int MODE>
+struct PairWalker {
+  const ExpertMmArgs& a;
+  const int32_t *start, *off;
+  int e, t;
+  __device__ PairWalker(const ExpertMmArgs& args, const int32_t* s, const int32_t* o) : a(args), start(s), off(o) {
+    e = 0;
+    t = (int)(blockIdx.x >> 1) - (int)(gridDim.x >> 1);
+  }
+  __device__ bool next(PairTile& k) {
+    t += gridDim.x >> 1;
+    const int E = a.E;
+    if (t >= start[E + 1]) return false;
+    while (t >= start[e + 1]) ++e;
+    const int rel = t - start[e], first = off[e], rows = (e < E ? off[e + 1] : a.P) - first;
+    const int tn = MODE == kGradW ? a.tiles_n : (rows + 255) / 256;
+    const int band = rel / (kBand * a.tiles_m), in = rel - band * kBand * a.tiles_m, h = min(kBand, tn - band * kBand);
+    k.e = e;
+    k.m = in / h;
+    k.n = band * kBand + in - k.m * h;
+    if (MODE == kGradW) {
+      k.row0 = first;
+      k.rows = rows;
+      k.nk = (rows + kTileK - 1) / kTileK;
+      k.cols = min(256, (a.N - k.n * 256 + 31) / 32 * 32);
+    } else {
+      // whole tiles, but the last two share what is left evenly (in steps of 32): a short last tile would cost its
+      // weights' loads, which take half the time of a whole tile
+      const int left = rows - (tn - 2) * 256, q = tn < 2 ? rows : min(256, ((left + 1) / 2 + 31) / 32 * 32);
+      const int at = tn < 2 || k.n < tn - 1 ? k.n * 256 : (tn - 2) * 256 + q;
+      k.row0 = first + at;
+      k.rows = k.n < tn - 2 ? 256 : k.n == tn - 1 ? rows - at : q;
+      k.cols = (k.rows + 31) / 32 * 32;
+      k.nk = e < E ? a.nk : 0;
     }
     return true;
   }
 };
 
-__device__ __forceinline__ float silu(float g) { return g / (1.f + __expf(-g)); }
-
-template <typename T, int MODE, bool GATED, int AM>
-__global__ void __launch_bounds__(kThreads, 1) expert_mm_kernel(const __grid_constant__ CUtensorMap tmA,
-                                                                const __grid_constant__ CUtensorMap tmB,
-                                                                const ExpertMmArgs a) {
-  using C = Cfg<AM>;
+template <typename T, int MODE, bool GATED>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    expert_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                       const __grid_constant__ CUtensorMap tmB64, const __grid_constant__ CUtensorMap tmB32,
+                       const ExpertMmArgs a) {
+  using C = Pair;
   constexpr int kStages = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (pm::smem_u32(smem_raw) & 1023)) & 1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
-  uint64_t* empty = full + kStages;
-  uint64_t* d_full = empty + kStages;  // [2]
-  uint64_t* d_empty = d_full + 2;      // [2]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);  // leader's: both CTAs' loads of a stage
+  uint64_t* empty = full + kMaxStages;       // each CTA's: the MMA has read its stage
+  uint64_t* tail = empty + kMaxStages;       // kGradW, each CTA's: loads of an expert's ragged last stage
+  uint64_t* peer_tail = tail + kMaxStages;   // leader's: the peer has zeroed its ragged rows
+  uint64_t* d_full = peer_tail + kMaxStages; // [2], each CTA's
+  uint64_t* d_empty = d_full + 2;            // [2], leader's: epilogue warps of both CTAs
   uint64_t* drain = d_empty + 2;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tslot + 1);
-  int32_t* off = reinterpret_cast<int32_t*>(smem + C::kBarOff + 256);
+  int32_t* off = reinterpret_cast<int32_t*>(smem + C::kTableOff);
   int32_t* start = off + a.E + 1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = (int)pm::cluster_ctarank();
 
   if (warp == 0) {
-    pm::tmem_alloc(tslot, 512);
-    pm::tmem_relinquish();
+    pm::tmem_alloc2(tslot, 512);
+    pm::tmem_relinquish2();
   }
   if (tid == 32) {
     for (int s = 0; s < kStages; ++s) {
       pm::mbar_init(full + s, 1);
       pm::mbar_init(empty + s, 1);
+      pm::mbar_init(tail + s, 1);
+      pm::mbar_init(peer_tail + s, 1);
     }
     for (int s = 0; s < 2; ++s) {
       pm::mbar_init(d_full + s, 1);
-      pm::mbar_init(d_empty + s, 4);
+      pm::mbar_init(d_empty + s, 2 * kEpiWarps);
     }
     pm::mbar_init(drain, 1);
     *abort_flag = 0;
     pm::fence_mbar_init();
   }
-  if (warp == 2) {
-    // offsets, clamped to 0 = off[0] <= off[e] <= off[e + 1] <= P (a wrong table must not reach memory), and tiles
-    int carry_off = 0, carry_t = 0;
-    for (int e0 = 0; e0 <= a.E; e0 += 32) {
-      const int e = e0 + lane;
-      int o = e > 0 && e <= a.E ? min(max(a.offsets[e], 0), a.P) : 0;
-#pragma unroll
-      for (int s = 1; s < 32; s <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, o, s);
-        if (lane >= s) o = max(o, u);
-      }
-      o = max(o, carry_off);
-      if (e <= a.E) off[e] = o;
-      carry_off = __shfl_sync(0xffffffffu, o, 31);
-    }
-    __syncwarp();
-    for (int e0 = 0; e0 <= a.E; e0 += 32) {
-      const int e = e0 + lane;
-      int c = 0;
-      if (e <= a.E) {
-        if (MODE == kGradW)
-          c = e < a.E ? a.tiles_m * a.tiles_n : 0;
-        else
-          c = ((e < a.E ? off[e + 1] : a.P) - off[e] + AM - 1) / AM * a.tiles_n;
-      }
-      int inc = c;
-#pragma unroll
-      for (int s = 1; s < 32; s <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, inc, s);
-        if (lane >= s) inc += u;
-      }
-      if (e <= a.E) start[e + 1] = carry_t + inc;
-      carry_t += __shfl_sync(0xffffffffu, inc, 31);
-    }
-    if (lane == 0) start[0] = 0;
-  }
+  if (warp == 2)
+    tile_table(a, off, start, lane, [&](int rows, int e) {
+      return MODE == kGradW ? (e < a.E ? a.tiles_m * a.tiles_n : 0) : (rows + 255) / 256 * a.tiles_m;
+    });
   pm::tc_fence_before();
   __syncthreads();
+  pm::cluster_sync();  // the peer's barriers exist
   pm::tc_fence_after();
   const uint32_t tmem = *tslot;
-  Walker<MODE, AM> walk(a, start, off);
-  Tile t;
+  PairWalker<MODE> walk(a, start, off);
+  PairTile t;
   // For converged warps: the same answer in every lane (tcgen05 instructions are warp-collective).
-  auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
-    const bool ok = __all_sync(0xffffffffu, pm::mbar_wait(bar, parity, lane == 0 ? a.err : nullptr, site));
+  auto agreed = [&](bool ok) {
+    ok = __all_sync(0xffffffffu, ok);
     if (!ok) *abort_flag = 1;
     return ok;
   };
+  auto site = [&] { return lane == 0 ? a.err : nullptr; };
   auto stopped = [&] { return __any_sync(0xffffffffu, *abort_flag != 0) != 0; };
 
   if (warp == 0) {
-    // ------------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      int st = 0, issued = 0;
-      uint32_t ph = 0, last_ph[kStages];
-      while (!*abort_flag && walk.next(t)) {
-        for (int i = 0; i < t.nk; ++i) {
-          if (!pm::mbar_wait(empty + st, ph ^ 1, a.err, 401)) {
-            *abort_flag = 1;
-            break;
-          }
-          uint8_t* sa = smem + st * C::kStageBytes;
-          uint8_t* sb = sa + C::kABytes;
-          pm::mbar_arrive_expect_tx(full + st, C::kStageBytes);
-          const int k0 = i * kTileK;
-          if (MODE == kGradW) {
-            const int r0 = t.row0 + k0;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) pm::tma_load_2d(sa + c * kChunk, &tmA, t.m * kTileM + 64 * c, r0, full + st);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) pm::tma_load_2d(sb + c * kChunk, &tmB, t.n * kTileN + 64 * c, r0, full + st);
+    // ------------------------------------------------------------------ TMA producer (each CTA its own halves)
+    int st = 0, issued = 0;
+    uint32_t ph = 0;
+    while (!stopped() && walk.next(t)) {
+      // B rows (kGradW: columns) of this CTA.  kForward, kGradX: at most two boxes, because each load costs the
+      // producer as much as 16 rows cost the transfer: 112 and 128 rows come as 128, 80 and 96 as 64 + 32,
+      // 48 and 64 as 64, less as 32.
+      const int half = t.cols >> 1;
+      const int parts = MODE == kGradW ? (half + 63) / 64 : half == 80 || half == 96 ? 2 : 1;
+      const uint32_t bytes = C::kABytes + (MODE == kGradW ? parts * kChunk : half > 96 ? kHalf : half > 64 ? 96 * 128 : half > 32 ? 64 * 128 : 32 * 128);
+      for (int i = 0; i < t.nk; ++i) {
+        if (!agreed(pm::mbar_wait(empty + st, ph ^ 1, site(), 401))) break;
+        uint8_t* sa = smem + st * C::kStageBytes;
+        uint8_t* sb = sa + C::kABytes;
+        const int k0 = i * kTileK;
+        uint32_t bar = pm::dsmem_addr(full + st, 0);
+        if (MODE == kGradW && t.rows - k0 < kTileK) {  // ragged rows: the loads of each CTA are its own
+          if (rank == 0) pm::mbar_arrive_expect_tx_warp(full + st, 0);
+          bar = pm::dsmem_addr(tail + st, rank);
+          pm::mbar_arrive_expect_tx_warp(tail + st, bytes);
+        } else if (rank == 0) {
+          pm::mbar_arrive_expect_tx_warp(full + st, 2 * bytes);
+        }
+        if (MODE == kGradW) {
+          const int r0 = t.row0 + k0, n0 = t.m * 256 + rank * 128, c0 = t.n * 256 + rank * half;
+          if (a.a_chunks == 2) {
+            pm::tma2_load_4d_warp(sa, &tmA, 0, r0, n0 >> 6, 0, bar);
           } else {
-            pm::tma_load_2d(sa, &tmA, k0, t.row0, full + st);
-            if (MODE == kForward && GATED)  // 128 gate rows, then the matching 128 up rows
-              pm::tma_load_4d(sb, &tmB, k0, t.n * (kTileN / 2), 0, t.e, full + st);
-            else if (MODE == kForward)
-              pm::tma_load_4d(sb, &tmB, k0, t.n * kTileN, t.e, 0, full + st);
-            else
-#pragma unroll
-              for (int c = 0; c < 4; ++c)
-                pm::tma_load_4d(sb + c * kChunk, &tmB, t.n * kTileN + 64 * c, k0, t.e, 0, full + st);
+            pm::tma2_load_4d_warp(sa, &tmA, n0, r0, 0, 0, bar);
+            pm::tma2_load_4d_warp(sa + kChunk, &tmA, n0 + 64, r0, 0, 0, bar);
           }
-          last_ph[st] = ph;
-          if (issued < kStages) ++issued;
-          if (++st == kStages) { st = 0; ph ^= 1; }
+          if (a.b_chunks == 2 && half == 128) {
+            pm::tma2_load_4d_warp(sb, &tmB, 0, r0, c0 >> 6, 0, bar);
+          } else {
+            pm::tma2_load_2d_warp(sb, &tmB64, c0, r0, bar);
+            if (parts > 1) pm::tma2_load_2d_warp(sb + kChunk, &tmB64, c0 + 64, r0, bar);
+          }
+        } else {
+          const int f0 = t.m * 256 + rank * 128;
+          if (MODE == kForward && GATED) {  // 8 groups of 8 gate rows and the matching 8 up rows
+            pm::tma2_load_5d_warp(sa, &tmA, k0, 0, 0, f0 >> 4, t.e, bar);
+          } else if (MODE == kForward) {
+            pm::tma2_load_4d_warp(sa, &tmA, k0, f0, t.e, 0, bar);
+          } else {
+            if (a.a_chunks == 2) {
+              pm::tma2_load_4d_warp(sa, &tmA, 0, k0, f0 >> 6, t.e, bar);
+            } else {
+              pm::tma2_load_4d_warp(sa, &tmA, f0, k0, 0, t.e, bar);
+              pm::tma2_load_4d_warp(sa + kChunk, &tmA, f0 + 64, k0, 0, t.e, bar);
+            }
+          }
+          const int r0 = t.row0 + rank * half;
+          if (half > 96)
+            pm::tma2_load_2d_warp(sb, &tmB, k0, r0, bar);
+          else if (half > 32)
+            pm::tma2_load_2d_warp(sb, &tmB64, k0, r0, bar);
+          else
+            pm::tma2_load_2d_warp(sb, &tmB32, k0, r0, bar);
+          if (parts == 2) pm::tma2_load_2d_warp(sb + 64 * 128, &tmB32, k0, r0 + 64, bar);
         }
+        if (issued < kStages) ++issued;
+        if (++st == kStages) { st = 0; ph ^= 1; }
       }
-      if (*abort_flag)  // let the copies in flight land before the CTA can exit
-        for (int j = 1; j <= issued; ++j) {
-          const int s = (st - j + kStages) % kStages;
-          pm::mbar_wait(full + s, last_ph[s], nullptr, 0, 20000000ull);
-        }
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer (converged warp)
-    const uint32_t idesc = pm::make_idesc_f16(kTileM, kTileN, sizeof(T) == 2 && a.half == 0 ? 1 : 0,
-                                              MODE == kGradW ? 1 : 0, MODE == kForward ? 0 : 1);
+    // Every load has landed once the MMA has read its stage: wait for the last ones, so that no copy into this
+    // CTA is in flight when it leaves.
+    const bool gone = stopped();
+    for (int j = 1; j <= issued; ++j) {
+      const int s = (st - j + kStages) % kStages;
+      pm::mbar_wait(empty + s, s < st ? ph : ph ^ 1, gone ? nullptr : site(), 406, gone ? 20000000ull : 2000000000ull);
+    }
+  } else if (warp == 1 && (rank == 0 || MODE == kGradW)) {
+    // ------------------------------------------------------------------ MMA issuer (leader), ragged rows (both)
     int st = 0, buf = 0;
-    uint32_t ph = 0, dph = 0;
+    uint32_t ph = 0, dph = 0, tail_ph = 0;
     while (!stopped() && walk.next(t)) {
       if (t.nk == 0) continue;
-      if (!wait(d_empty + buf, dph ^ 1, 402)) break;
-      pm::tc_fence_after();
-      const uint32_t d = tmem + buf * kTileN;
+      if (rank == 0) {
+        if (!agreed(pm::mbar_wait_cluster(d_empty + buf, dph ^ 1, site(), 402))) break;
+        pm::tc_fence_after();
+      }
+      const uint32_t idesc = pm::make_idesc_f16(256, t.cols, a.half ? 0 : 1, MODE == kForward ? 0 : 1, MODE == kGradW ? 1 : 0);
+      const uint32_t d = tmem + buf * 256;
       bool ok = true;
-      for (int i = 0; i < t.nk; ++i) {
-        ok = wait(full + st, ph, 403);
-        if (!ok) break;
+      for (int i = 0; i < t.nk && ok; ++i) {
+        if (rank == 0) ok = agreed(pm::mbar_wait(full + st, ph, site(), 403));
         uint8_t* sp = smem + st * C::kStageBytes;
         int steps = 4;
-        if (MODE == kGradW && t.rows - i * kTileK < kTileK) {
-          // the expert's last stage: its steps of 16 rows, the last of them completed with zero rows
+        if (MODE == kGradW && ok && t.rows - i * kTileK < kTileK) {
+          // steps of 16 rows, the last of them completed with zero rows (every column chunk of the stage)
+          ok = agreed(pm::mbar_wait(tail + st, (tail_ph >> st) & 1, site(), 407));
           const int have = t.rows - i * kTileK;
           steps = (have + 15) / 16;
-          const int pad = steps * 16 - have;
-          for (int j = lane; j < pad * 6 * 8; j += 32) {
+          const int pad = steps * 16 - have, chunks = 2 + ((t.cols >> 1) + 63) / 64;
+          for (int j = lane; j < pad * chunks * 8; j += 32) {
             const int chunk = j / (pad * 8), in = j - chunk * pad * 8, r = have + in / 8;
             *reinterpret_cast<uint4*>(sp + chunk * kChunk + r * 128 + (in & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           pm::fence_proxy_async_smem();
           __syncwarp();
+          if (rank == 1) {
+            if (lane == 0) pm::mbar_arrive_cluster(pm::dsmem_addr(peer_tail + st, 0));
+          } else if (ok) {
+            ok = agreed(pm::mbar_wait_cluster(peer_tail + st, (tail_ph >> st) & 1, site(), 408));
+          }
+          tail_ph ^= 1u << st;
         }
-        pm::tc_fence_after();
-        const uint32_t sa = pm::smem_u32(sp), sb = sa + C::kABytes;
+        if (rank == 0 && ok) {
+          pm::tc_fence_after();
+          const uint32_t sa = pm::smem_u32(sp), sb = sa + C::kABytes;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (MODE == kGradW && k >= steps) break;
-          const uint64_t ad = MODE == kGradW ? pm::make_sdesc(sa + k * 2048, kChunk, 1024)
-                                             : pm::make_sdesc(sa + 32 * k, 16, 1024);
-          const uint64_t bd = MODE == kForward ? pm::make_sdesc(sb + 32 * k, 16, 1024)
-                                               : pm::make_sdesc(sb + k * 2048, kChunk, 1024);
-          pm::umma_f16_warp(d, ad, bd, idesc, (i | k) ? 1u : 0u);
+          for (int k = 0; k < 4; ++k) {
+            if (MODE == kGradW && k >= steps) break;
+            const uint64_t bd = MODE == kGradW ? pm::make_sdesc(sb + k * 2048, kChunk, 1024)
+                                               : pm::make_sdesc(sb + 32 * k, 16, 1024);
+            const uint64_t ad = MODE == kForward ? pm::make_sdesc(sa + 32 * k, 16, 1024)
+                                                 : pm::make_sdesc(sa + k * 2048, kChunk, 1024);
+            pm::umma2_f16_warp(d, ad, bd, idesc, (i | k) ? 1u : 0u);
+          }
+          pm::umma2_commit_both_warp(empty + st);
         }
-        pm::umma_commit_warp(empty + st);
         if (++st == kStages) { st = 0; ph ^= 1; }
       }
       if (!ok) break;
-      pm::umma_commit_warp(d_full + buf);
+      if (rank == 0) pm::umma2_commit_both_warp(d_full + buf);
       buf ^= 1;
       if (buf == 0) dph ^= 1;
     }
-    pm::umma_commit_warp(drain);  // arrives once every MMA issued above has completed
-    pm::mbar_wait(drain, 0, lane == 0 ? a.err : nullptr, 404);
-  } else {
-    // ------------------------------------------------------------------ epilogue (warps 2-5)
-    const int q = warp & 3;
+    if (rank == 0) {
+      pm::umma2_commit_both_warp(drain);  // arrives once every MMA issued above has completed
+      pm::mbar_wait(drain, 0, site(), 404);
+    }
+  } else if (warp >= 2) {
+    // ------------------------------------------------------------------ epilogue (warps 2-9 of both CTAs)
+    const int q = warp & 3, side = (warp - 2) >> 2;  // TMEM lane quadrant; half of the columns
     uint8_t* stage = smem + C::kEpiOff + (warp - 2) * kEpiWarpBytes;
     int buf = 0;
     uint32_t dph = 0;
-    // One output row is `ld` elements; columns [c0, c0 + 64) of it, as far as `cols` reaches
-    auto emit = [&](T* out, int64_t ld, int rows_here, int c0, int cols, const uint4 (&v)[8]) {
+    // y^T: lane = feature, v[i] = row i of 32.  Through shared memory [32 rows][32 features], then 64 bytes of a
+    // row by 4 lanes: eight rows an instruction.  `out`: the first row's first feature of this warp.
+    auto emit_t = [&](T* out, int64_t ld, int rows_here, int feats, const float (&v)[32]) {
 #pragma unroll
-      for (int u = 0; u < 8; ++u) *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ (lane & 7)) << 4)) = v[u];
+      for (int i = 0; i < 32; ++i) *reinterpret_cast<T*>(stage + i * 64 + lane * 2) = rows::from_f<T>(v[i]);
       __syncwarp();
-      // 8 lanes write the 128 bytes of a row: whole lines, four rows an instruction
-      const int u = lane & 7;
+      const int u = lane & 3;
 #pragma unroll
-      for (int g = 0; g < 8; ++g) {
-        const int r = g * 4 + (lane >> 3);
-        const uint4 w = *reinterpret_cast<const uint4*>(stage + r * 128 + ((u ^ (r & 7)) << 4));
-        if (r < rows_here && c0 + u * 8 < cols) *reinterpret_cast<uint4*>(out + r * ld + c0 + u * 8) = w;
+      for (int g = 0; g < 4; ++g) {
+        const int r = g * 8 + (lane >> 2);
+        const uint4 w = *reinterpret_cast<const uint4*>(stage + r * 64 + u * 16);
+        if (r < rows_here && u * 8 < feats) *reinterpret_cast<uint4*>(out + r * ld + u * 8) = w;
       }
       __syncwarp();
     };
-    auto pack = [&](const float* f, uint4 (&v)[8]) {
+    // The same for [gate | up] rows of ld elements: units of 8 lanes go to the gate and the up half by turns.
+    auto emit_pre = [&](T* out, int64_t ld, int up_off, int rows_here, int feats, const float (&v)[32]) {
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-        v[u] = make_uint4(rows::pack2<T>(f[8 * u], f[8 * u + 1]), rows::pack2<T>(f[8 * u + 2], f[8 * u + 3]),
-                          rows::pack2<T>(f[8 * u + 4], f[8 * u + 5]), rows::pack2<T>(f[8 * u + 6], f[8 * u + 7]));
+      for (int i = 0; i < 32; ++i) *reinterpret_cast<T*>(stage + i * 64 + lane * 2) = rows::from_f<T>(v[i]);
+      __syncwarp();
+      const int u = lane & 3;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int r = g * 8 + (lane >> 2);
+        const uint4 w = *reinterpret_cast<const uint4*>(stage + r * 64 + u * 16);
+        if (r < rows_here && u * 8 < feats) *reinterpret_cast<uint4*>(out + r * ld + (u & 1) * up_off + (u >> 1) * 8) = w;
+      }
+      __syncwarp();
+    };
+    // silu(gate) up: 32 rows of 16 features; lane 16 j + f (gate) has rows 0-15 and lane 16 j + 8 + f rows 16-31 of
+    // feature 8 j + f.
+    auto emit_gated = [&](T* out, int64_t ld, int rows_here, int feats, const float (&o)[16]) {
+      uint8_t* mine = stage + ((lane >> 3) & 1) * 16 * 32 + ((lane >> 4) * 8 + (lane & 7)) * 2;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) *reinterpret_cast<T*>(mine + i * 32) = rows::from_f<T>(o[i]);
+      __syncwarp();
+      const int u = lane & 1;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int r = g * 16 + (lane >> 1);
+        const uint4 w = *reinterpret_cast<const uint4*>(stage + r * 32 + u * 16);
+        if (r < rows_here && u * 8 < feats) *reinterpret_cast<uint4*>(out + r * ld + u * 8) = w;
+      }
+      __syncwarp();
     };
     while (!stopped() && walk.next(t)) {
       const bool zero = t.nk == 0;
       if (!zero) {
-        if (!wait(d_full + buf, dph, 405)) break;
+        if (!agreed(pm::mbar_wait(d_full + buf, dph, site(), 405))) break;
         pm::tc_fence_after();
       }
-      const uint32_t td = tmem + buf * kTileN + ((uint32_t)(32 * q) << 16);
-      const int lim = MODE == kGradW ? a.M - t.m * kTileM : t.rows;  // rows of the tile that exist
-      const int here = min(32, lim - 32 * q);
-      if (here > 0) {
-        const int64_t row = (MODE == kGradW ? (int64_t)t.e * a.M + t.m * kTileM : (int64_t)t.row0) + 32 * q;
-        uint4 v[8];
-        if (GATED) {
-          const int I = a.N / 2;
+      const uint32_t td = tmem + buf * 256 + ((uint32_t)(32 * q) << 16);
+      if (MODE == kGradW) {
+        // lane = n, columns = k: 32 columns a time, written as 64 bytes of a row by 4 lanes
+        const int n0 = t.m * 256 + rank * 128 + 32 * q, here = min(32, a.M - n0);
+        T* out = static_cast<T*>(a.out) + ((int64_t)t.e * a.M + n0) * a.N;
+        if (here > 0) {
 #pragma unroll 1
-          for (int c = 0; c < kTileN / 2; c += 64) {
-            const int c0 = t.n * (kTileN / 2) + c;
-            float g[64], u[64];
+          for (int c = side * 128; c < side * 128 + 128 && c < t.cols; c += 32) {
+            float f[32];
             if (zero) {
 #pragma unroll
-              for (int i = 0; i < 64; ++i) g[i] = u[i] = 0.f;
+              for (int i = 0; i < 32; ++i) f[i] = 0.f;
             } else {
-              pm::tmem_ld32(td + c, *reinterpret_cast<float(*)[32]>(g));
-              pm::tmem_ld32(td + c + 32, *reinterpret_cast<float(*)[32]>(g + 32));
-              pm::tmem_ld32(td + c + 128, *reinterpret_cast<float(*)[32]>(u));
-              pm::tmem_ld32(td + c + 160, *reinterpret_cast<float(*)[32]>(u + 32));
+              pm::tmem_ld32(td + c, f);
             }
-            if (a.pre) {  // the products themselves, for the backward pass
-              T* pr = static_cast<T*>(a.pre) + row * a.N;
-              pack(g, v);
-              emit(pr, a.N, here, c0, I, v);
-              pack(u, v);
-              emit(pr + I, a.N, here, c0, I, v);
-            }
+            // 16-byte units of a row permuted by row / 2: conflict-free both ways
 #pragma unroll
-            for (int i = 0; i < 64; ++i) g[i] = silu(g[i]) * u[i];
-            pack(g, v);
-            emit(static_cast<T*>(a.out) + row * I, I, here, c0, I, v);
+            for (int u = 0; u < 4; ++u)
+              *reinterpret_cast<uint4*>(stage + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) =
+                  make_uint4(rows::pack2<T>(f[8 * u], f[8 * u + 1]), rows::pack2<T>(f[8 * u + 2], f[8 * u + 3]),
+                             rows::pack2<T>(f[8 * u + 4], f[8 * u + 5]), rows::pack2<T>(f[8 * u + 6], f[8 * u + 7]));
+            __syncwarp();
+            const int u = lane & 3, col = t.n * 256 + c + u * 8;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int r = g * 8 + (lane >> 2);
+              const uint4 w = *reinterpret_cast<const uint4*>(stage + r * 64 + ((u ^ ((r >> 1) & 3)) << 4));
+              if (r < here && col < a.N) *reinterpret_cast<uint4*>(out + (int64_t)r * a.N + col) = w;
+            }
+            __syncwarp();
           }
-        } else {
-          T* out = static_cast<T*>(a.out) + row * a.N;
+        }
+      } else {
+        const int f0 = t.m * 256 + rank * 128 + 32 * q, feats = a.N - f0;  // of W's rows; gated: 16 gates and 16 ups
+        if (feats > 0) {
 #pragma unroll 1
-          for (int c = 0; c < kTileN; c += 64) {
-            float f[64];
+          for (int c = side * 32; c < t.rows; c += 64) {
+            const int64_t row = (int64_t)t.row0 + c;
+            const int here = t.rows - c;
+            float v[32];
             if (zero) {
 #pragma unroll
-              for (int i = 0; i < 64; ++i) f[i] = 0.f;
+              for (int i = 0; i < 32; ++i) v[i] = 0.f;
             } else {
-              pm::tmem_ld32(td + c, *reinterpret_cast<float(*)[32]>(f));
-              pm::tmem_ld32(td + c + 32, *reinterpret_cast<float(*)[32]>(f + 32));
+              pm::tmem_ld32(td + c, v);
             }
-            pack(f, v);
-            emit(out, a.N, here, t.n * kTileN + c, a.N, v);
+            if (!GATED) {
+              emit_t(static_cast<T*>(a.out) + row * a.N + f0, a.N, here, feats, v);
+              continue;
+            }
+            // the products themselves, for the backward pass: lanes 8 j .. 8 j + 7 are gates (j even) or ups
+            const int I = a.N / 2, up = (lane >> 3) & 1;
+            if (a.pre) emit_pre(static_cast<T*>(a.pre) + row * a.N + (f0 >> 1), a.N, I, here, feats, v);
+            // lanes 8 apart trade halves: a gate lane then has rows 0-15 of both products, an up lane rows 16-31
+            float o[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float got = __shfl_xor_sync(0xffffffffu, up ? v[i] : v[16 + i], 8);
+              o[i] = up ? silu(got) * v[16 + i] : silu(v[i]) * got;
+            }
+            emit_gated(static_cast<T*>(a.out) + row * I + (f0 >> 1), I, here, feats >> 1, o);
           }
         }
       }
       if (!zero) {
         pm::tc_fence_before();
         __syncwarp();
-        if (lane == 0) pm::mbar_arrive(d_empty + buf);
+        if (lane == 0) pm::mbar_arrive_cluster_relaxed(pm::dsmem_addr(d_empty + buf, 0));
         buf ^= 1;
         if (buf == 0) dph ^= 1;
       }
@@ -372,7 +461,9 @@ __global__ void __launch_bounds__(kThreads, 1) expert_mm_kernel(const __grid_con
   }
   pm::tc_fence_before();
   __syncthreads();
-  if (warp == 0) pm::tmem_dealloc(tmem, 512);
+  pm::cluster_sync();  // no CTA leaves while its peer may still signal it or read its operands
+  pm::tc_fence_after();
+  if (warp == 0) pm::tmem_dealloc2(tmem, 512);
 }
 
 // ----------------------------------------------------------------------------- SwiGLU gradient
@@ -408,24 +499,28 @@ __global__ void __launch_bounds__(256) swiglu_bwd_kernel(const T* __restrict__ d
   }
 }
 
-template <typename T, int MODE, bool GATED, int AM>
-int launch_mm(const CUtensorMap& ta, const CUtensorMap& tb, const ExpertMmArgs& a, cudaStream_t stream) {
-  const int smem = (int)(Cfg<AM>::kFixed + (2 * a.E + 3) * sizeof(int32_t));
-  if (smem > 232448) return -2;
-  auto* fn = expert_mm_kernel<T, MODE, GATED, AM>;
+constexpr int kMaxSmem = 232448;
+
+template <typename T, int MODE, bool GATED>
+int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb64, const CUtensorMap& tb32, const ExpertMmArgs& a,
+                cudaStream_t stream) {
+  const int smem = (int)(Pair::kFixed + (2 * a.E + 3) * sizeof(int32_t));
+  if (smem > kMaxSmem) return -2;
+  auto* fn = expert_pair_kernel<T, MODE, GATED>;
   cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  fn<<<a.num_sms, kThreads, smem, stream>>>(ta, tb, a);
+  fn<<<a.num_sms / 2 * 2, kPairThreads, smem, stream>>>(ta, tb, tb64, tb32, a);
   return 0;
 }
-
 template <typename T>
-int launch_mode(int mode, bool gated, bool few, const CUtensorMap& ta, const CUtensorMap& tb, const ExpertMmArgs& a,
-                cudaStream_t s) {
-  if (mode == kGradW) return launch_mm<T, kGradW, false, 128>(ta, tb, a, s);
-  if (mode == kGradX) return launch_mm<T, kGradX, false, 128>(ta, tb, a, s);
-  if (gated) return few ? launch_mm<T, kForward, true, 32>(ta, tb, a, s) : launch_mm<T, kForward, true, 128>(ta, tb, a, s);
-  return few ? launch_mm<T, kForward, false, 32>(ta, tb, a, s) : launch_mm<T, kForward, false, 128>(ta, tb, a, s);
+int launch_mode(int mode, bool gated, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb64,
+                const CUtensorMap& tb32, const ExpertMmArgs& a, cudaStream_t s) {
+  if (mode == kGradW) return launch_pair<T, kGradW, false>(ta, tb, tb64, tb32, a, s);
+  if (mode == kGradX) return launch_pair<T, kGradX, false>(ta, tb, tb64, tb32, a, s);
+  return gated ? launch_pair<T, kForward, true>(ta, tb, tb64, tb32, a, s)
+               : launch_pair<T, kForward, false>(ta, tb, tb64, tb32, a, s);
 }
+
+int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 }  // namespace
 
@@ -441,48 +536,57 @@ int launch_expert_mm(int mode, const ExpertMmCall& c, cudaStream_t stream) {
   a.half = c.half;
   a.num_sms = c.num_sms;
   a.err = c.err;
-  const uint64_t K = c.K, N = c.N, E = c.E, P = c.P;
-  const bool few = mode == kForward && c.P <= (int64_t)32 * c.E;
-  CUtensorMap ta, tb;
+  const uint64_t K = c.K, N = c.N, E = c.E, P = c.P, I = N / 2;
+  CUtensorMap ta, tb, tb64, tb32;  // A; B in boxes of 128, 64 and 32 rows (kGradW: two chunks, or one)
+  const uint64_t dx[2] = {K, P}, sx[1] = {(uint64_t)c.xs * 2}, dd[2] = {N, P}, sd[1] = {(uint64_t)c.dzs * 2};
+  const uint64_t dw[4] = {K, N, E, 1}, sw[3] = {K * 2, N * K * 2, E * N * K * 2};
+  // gated weights: [E][I / 8][gate | up][8][K]
+  const uint64_t dg[5] = {K, 8, 2, I / 8, E}, sg[4] = {K * 2, I * K * 2, 8 * K * 2, N * K * 2};
   int rc;
-  if (mode == kForward) {
-    const uint64_t da[2] = {K, P}, sa[1] = {(uint64_t)c.xs * 2};
-    const uint32_t ba[2] = {kTileK, few ? 32u : 128u};
-    rc = make_tmap_16b_sw128(&ta, c.x, 2, da, sa, ba, c.half);
-    if (c.gated) {
-      const uint64_t db[4] = {K, N / 2, 2, E}, sb[3] = {K * 2, N / 2 * K * 2, N * K * 2};
-      const uint32_t bb[4] = {kTileK, 128, 2, 1};
-      if (!rc) rc = make_tmap_16b_sw128(&tb, c.w, 4, db, sb, bb, c.half);
-    } else {
-      const uint64_t db[4] = {K, N, E, 1}, sb[3] = {K * 2, N * K * 2, E * N * K * 2};
-      const uint32_t bb[4] = {kTileK, 256, 1, 1};
-      if (!rc) rc = make_tmap_16b_sw128(&tb, c.w, 4, db, sb, bb, c.half);
-    }
-    a.N = (int)N;
-    a.nk = (int)((K + kTileK - 1) / kTileK);
-    a.tiles_n = (int)(((c.gated ? N / 2 : N) + (c.gated ? 127 : 255)) / (c.gated ? 128 : 256));
-  } else {
-    const uint64_t da[2] = {N, P}, sa[1] = {(uint64_t)c.dzs * 2};
-    const uint32_t ba[2] = {kTileK, mode == kGradX ? 128u : 64u};
-    rc = make_tmap_16b_sw128(&ta, c.dz, 2, da, sa, ba, c.half);
+  // MN-major operands [stack][rows][width]: one box of 64 rows x 2 chunks of 64 columns, where the chunks of a row
+  // can be a dimension of the tensor (64 divides the width); else a box for each chunk
+  auto chunked = [&](CUtensorMap* m, const void* p, uint64_t width, uint64_t rows, uint64_t stride, uint64_t stack, int* n) {
+    *n = width % 64 == 0 ? 2 : 1;
+    const uint64_t wide = width / 64, whole = stack > 1 ? rows * stride : 16;
+    const uint64_t d2[4] = {64, rows, wide, stack}, s2[3] = {stride, 128, whole};
+    const uint64_t d1[4] = {width, rows, 1, stack}, s1[3] = {stride, 16, whole};
+    const uint32_t b2[4] = {64, kTileK, 2, 1}, b1[4] = {64, kTileK, 1, 1};
+    return *n == 2 ? make_tmap_16b_sw128(m, p, 4, d2, s2, b2, c.half) : make_tmap_16b_sw128(m, p, 4, d1, s1, b1, c.half);
+  };
+  if (mode == kGradW) {
+    const uint32_t box[2] = {64, kTileK};
+    rc = chunked(&ta, c.dz, N, P, (uint64_t)c.dzs * 2, 1, &a.a_chunks);
+    if (!rc) rc = chunked(&tb, c.x, K, P, (uint64_t)c.xs * 2, 1, &a.b_chunks);
+    if (!rc) rc = make_tmap_16b_sw128(&tb64, c.x, 2, dx, sx, box, c.half);
+    tb32 = tb64;
     a.N = (int)K;
-    a.tiles_n = (int)((K + kTileN - 1) / kTileN);
-    if (mode == kGradX) {
-      const uint64_t db[4] = {K, N, E, 1}, sb[3] = {K * 2, N * K * 2, E * N * K * 2};
-      const uint32_t bb[4] = {64, kTileK, 1, 1};
-      if (!rc) rc = make_tmap_16b_sw128(&tb, c.w, 4, db, sb, bb, c.half);
-      a.nk = (int)((N + kTileK - 1) / kTileK);
+    a.M = (int)N;
+    a.tiles_m = ceil_div(N, 256);
+    a.tiles_n = ceil_div(K, 256);
+  } else {
+    const void* r = mode == kForward ? c.x : c.dz;
+    const uint64_t *dr = mode == kForward ? dx : dd, *sr = mode == kForward ? sx : sd;
+    const uint32_t box128[2] = {kTileK, 128}, box64[2] = {kTileK, 64}, box32[2] = {kTileK, 32};
+    rc = make_tmap_16b_sw128(&tb, r, 2, dr, sr, box128, c.half);
+    if (!rc) rc = make_tmap_16b_sw128(&tb64, r, 2, dr, sr, box64, c.half);
+    if (!rc) rc = make_tmap_16b_sw128(&tb32, r, 2, dr, sr, box32, c.half);
+    if (c.gated) {
+      const uint32_t box[5] = {kTileK, 8, 2, 8, 1};
+      if (!rc) rc = make_tmap_16b_sw128(&ta, c.w, 5, dg, sg, box, c.half);
+    } else if (mode == kGradX) {
+      if (!rc) rc = chunked(&ta, c.w, K, N, K * 2, E, &a.a_chunks);
     } else {
-      const uint64_t db[2] = {K, P}, sb[1] = {(uint64_t)c.xs * 2};
-      const uint32_t bb[2] = {64, kTileK};
-      if (!rc) rc = make_tmap_16b_sw128(&tb, c.x, 2, db, sb, bb, c.half);
-      a.M = (int)N;
-      a.tiles_m = (int)((N + kTileM - 1) / kTileM);
+      const uint32_t box[4] = {64, 128u, 1, 1};
+      if (!rc) rc = make_tmap_16b_sw128(&ta, c.w, 4, dw, sw, box, c.half);
     }
+    a.N = (int)(mode == kForward ? N : K);
+    a.nk = ceil_div(mode == kForward ? K : N, kTileK);
+    const int64_t features = mode == kGradX ? K : c.gated ? I : N;
+    a.tiles_m = ceil_div(features, c.gated ? 128 : 256);
   }
   if (rc) return rc;
-  return c.half ? launch_mode<__half>(mode, c.gated, few, ta, tb, a, stream)
-                : launch_mode<__nv_bfloat16>(mode, c.gated, few, ta, tb, a, stream);
+  return c.half ? launch_mode<__half>(mode, c.gated, ta, tb, tb64, tb32, a, stream)
+                : launch_mode<__nv_bfloat16>(mode, c.gated, ta, tb, tb64, tb32, a, stream);
 }
 
 void launch_swiglu_bwd(const void* da, int64_t das, const void* z, int64_t zs, void* dz, int64_t P, int I,

@@ -339,6 +339,7 @@ void launch_expert_combine_bwd(const CombineBwdArgs& a, int type, bool out_f32, 
 struct ExpertMmArgs {
   int E, P, N, M;         // N: output row stride (kForward gated: 2 I); M: output rows of an expert (kGradW)
   int nk, tiles_m, tiles_n, num_sms, half;
+  int a_chunks, b_chunks; // 64-column chunks that one load of an MN-major operand brings (1 or 2)
   const int32_t* offsets;
   void* out;
   void* pre;
