@@ -529,42 +529,114 @@ __device__ __forceinline__ void umma2_commit_both_warp(uint64_t* bar) {
       "h"((uint16_t)3)
       : "memory");
 }
-// Tiled loads into this CTA's shared memory that complete on a barrier of either CTA of the pair
-// (`bar_cluster` from dsmem_addr); no multicast.  Warp-collective: one elected lane of a converged warp issues
-// (from a single divergent lane each load costs the issuing thread over 100 cycles, as for the MMA forms).
-__device__ __forceinline__ void tma2_load_2d_warp(void* smem_dst, const void* tmap, int x, int y, uint32_t bar_cluster) {
+// Pair loads into this CTA's shared memory (addresses from smem_u32) that complete on a barrier of either CTA of the
+// pair (`bar` from dsmem_addr); no multicast.  Warp-collective: one elected lane of a converged warp issues (from a
+// single divergent lane each load costs the issuing thread over 100 cycles, as for the MMA forms).
+__device__ __forceinline__ void tma2_load_2d_warp(uint32_t dst, const void* tmap, int x, int y, uint32_t bar) {
   asm volatile(
       "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
       "@e cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
-      "%3}], [%4];\n\t}" ::"r"(smem_u32(smem_dst)),
-      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(bar_cluster)
+      "%3}], [%4];\n\t}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ void tma2_load_4d_warp(void* smem_dst, const void* tmap, int x, int y, int z, int w,
-                                                  uint32_t bar_cluster) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-      "@e cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
-      "%3, %4, %5}], [%6];\n\t}" ::"r"(smem_u32(smem_dst)),
-      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar_cluster)
-      : "memory");
-}
-__device__ __forceinline__ void tma2_load_5d_warp(void* smem_dst, const void* tmap, int x, int y, int z, int w, int v,
-                                                  uint32_t bar_cluster) {
+__device__ __forceinline__ void tma2_load_5d_warp(uint32_t dst, const void* tmap, int x, int y, int z, int w, int v,
+                                                  uint32_t bar) {
   asm volatile(
       "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
       "@e cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
-      "%3, %4, %5, %6}], [%7];\n\t}" ::"r"(smem_u32(smem_dst)),
-      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v), "r"(bar_cluster)
+      "%3, %4, %5, %6}], [%7];\n\t}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v), "r"(bar)
       : "memory");
 }
-// The same for arrivals on this CTA's barriers.
-__device__ __forceinline__ void mbar_arrive_expect_tx_warp(uint64_t* bar, uint32_t bytes) {
+// A stage of two loads (5-D, and 2-D or 5-D) by one election: the issuing warp's instructions, not the copies,
+// bound short stages.
+__device__ __forceinline__ void tma2_stage_52_warp(uint32_t a, const void* ma, int x, int y, int z, int w, int v, uint32_t b,
+                                                   const void* mb, int bx, int by, uint32_t bar) {
   asm volatile(
       "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-      "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(smem_u32(bar)),
+      "@e cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3, %4, %5, %6}], [%11];\n\t"
+      "@e cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%7], [%8, {%9, "
+      "%10}], [%11];\n\t}" ::"r"(a),
+      "l"(reinterpret_cast<uint64_t>(ma)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v), "r"(b),
+      "l"(reinterpret_cast<uint64_t>(mb)), "r"(bx), "r"(by), "r"(bar)
+      : "memory");
+}
+// (both 5-D maps with coordinates {0, y, z or bz, 0, 0})
+__device__ __forceinline__ void tma2_stage_55_warp(uint32_t a, const void* ma, int y, int z, uint32_t b, const void* mb,
+                                                   int bz, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%8, "
+      "%2, %3, %8, %8}], [%7];\n\t"
+      "@e cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%4], [%5, {%8, "
+      "%2, %6, %8, %8}], [%7];\n\t}" ::"r"(a),
+      "l"(reinterpret_cast<uint64_t>(ma)), "r"(y), "r"(z), "r"(b), "l"(reinterpret_cast<uint64_t>(mb)), "r"(bz), "r"(bar),
+      "r"(0)
+      : "memory");
+}
+// Arrive on this CTA's barrier (address from smem_u32), expecting bytes.
+__device__ __forceinline__ void mbar_arrive_expect_tx_warp(uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
       "r"(bytes)
       : "memory");
+}
+// A stage of four MMAs (64 of K): descriptors advance by AS and BS (16-byte units) between them, then the commit of
+// umma2_commit_both_warp; one election.
+template <int AS, int BS>
+__device__ __forceinline__ void umma2_f16_stage_warp(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                     uint32_t accumulate, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred e, p, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+      "add.u64 a1, %1, %6;\n\tadd.u64 a2, %1, %7;\n\tadd.u64 a3, %1, %8;\n\t"
+      "add.u64 b1, %2, %9;\n\tadd.u64 b2, %2, %10;\n\tadd.u64 b3, %2, %11;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a1, b1, %3, t;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a2, b2, %3, t;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a3, b3, %3, t;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%5], %12;\n\t}" ::
+          "r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(bar), "n"(AS), "n"(2 * AS), "n"(3 * AS), "n"(BS),
+      "n"(2 * BS), "n"(3 * BS), "h"((uint16_t)3)
+      : "memory");
+}
+// Bounded wait of a converged warp on this CTA's barrier (address from smem_u32): the same answer in every lane.
+// CLUSTER: acquires at cluster scope, for barriers that other CTAs' threads arrive on.
+template <bool CLUSTER>
+__device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity, uint32_t hint_ns) {
+  uint32_t ok;
+  if (CLUSTER)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(hint_ns)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(hint_ns)
+        : "memory");
+  return ok != 0;
+}
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, int* err, int site,
+                                               uint64_t timeout_ns = 2000000000ull) {
+  if (__all_sync(0xffffffffu, mbar_poll<CLUSTER>(bar, parity, 10000u))) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (!__all_sync(0xffffffffu, mbar_poll<CLUSTER>(bar, parity, 100000u))) {
+    if (__any_sync(0xffffffffu, globaltimer_ns() - t0 > timeout_ns)) {
+      if ((threadIdx.x & 31) == 0) report_error(err, kWaitTimeout, site);
+      return false;
+    }
+  }
+  return true;
 }
 // Arrive on a barrier of any CTA of the cluster: releasing this thread's writes to the cluster, or (relaxed) only
 // counting, where what must be ordered is ordered by tcgen05 fences; a release waits for the thread's global
@@ -574,25 +646,6 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar_cluster
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
-}
-// mbar_wait that acquires at cluster scope: for barriers that other CTAs' threads arrive on.
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int* err, int site,
-                                                  uint64_t timeout_ns = 2000000000ull) {
-  const uint64_t t0 = globaltimer_ns();
-  for (;;) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(100000u)
-        : "memory");
-    if (ok) return true;
-    if (globaltimer_ns() - t0 > timeout_ns) break;
-  }
-  report_error(err, kWaitTimeout, site);
-  return false;
 }
 
 // ----------------------------------------------------------------------------- conversions

@@ -187,17 +187,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   const uint32_t tmem = *tslot;
   PairWalker<MODE> walk(a, start, off);
   PairTile t;
-  // For converged warps: the same answer in every lane (tcgen05 instructions are warp-collective).
-  auto agreed = [&](bool ok) {
-    ok = __all_sync(0xffffffffu, ok);
-    if (!ok) *abort_flag = 1;
-    return ok;
+  auto wait = [&](uint32_t bar, uint32_t parity, int site) {
+    if (pm::mbar_wait_warp(bar, parity, a.err, site)) return true;
+    *abort_flag = 1;
+    return false;
   };
-  auto site = [&] { return lane == 0 ? a.err : nullptr; };
+  auto wait_cluster = [&](uint32_t bar, uint32_t parity, int site) {
+    if (pm::mbar_wait_warp<true>(bar, parity, a.err, site)) return true;
+    *abort_flag = 1;
+    return false;
+  };
   auto stopped = [&] { return __any_sync(0xffffffffu, *abort_flag != 0) != 0; };
+  const uint32_t base = pm::smem_u32(smem), full_at = pm::smem_u32(full), empty_at = pm::smem_u32(empty);
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (each CTA its own halves)
+    const uint32_t full_leader = pm::dsmem_addr(full, 0);
     int st = 0, issued = 0;
     uint32_t ph = 0;
     while (!stopped() && walk.next(t)) {
@@ -207,56 +212,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const int half = t.cols >> 1;
       const int parts = MODE == kGradW ? (half + 63) / 64 : half == 80 || half == 96 ? 2 : 1;
       const uint32_t bytes = C::kABytes + (MODE == kGradW ? parts * kChunk : half > 96 ? kHalf : half > 64 ? 96 * 128 : half > 32 ? 64 * 128 : 32 * 128);
+      const CUtensorMap* mb = half > 96 ? &tmB : half > 32 ? &tmB64 : &tmB32;
+      const int f0 = t.m * 256 + rank * 128, r0 = t.row0 + rank * half, c0 = t.n * 256 + rank * half;
+      const bool simple = MODE == kForward || (a.a_chunks == 2 && (MODE == kGradX || (a.b_chunks == 2 && half == 128)));
       for (int i = 0; i < t.nk; ++i) {
-        if (!agreed(pm::mbar_wait(empty + st, ph ^ 1, site(), 401))) break;
-        uint8_t* sa = smem + st * C::kStageBytes;
-        uint8_t* sb = sa + C::kABytes;
+        if (!wait(empty_at + 8 * st, ph ^ 1, 401)) break;
+        const uint32_t sa = base + st * C::kStageBytes, sb = sa + C::kABytes;
         const int k0 = i * kTileK;
-        uint32_t bar = pm::dsmem_addr(full + st, 0);
+        uint32_t bar = full_leader + 8 * st;
         if (MODE == kGradW && t.rows - k0 < kTileK) {  // ragged rows: the loads of each CTA are its own
-          if (rank == 0) pm::mbar_arrive_expect_tx_warp(full + st, 0);
+          if (rank == 0) pm::mbar_arrive_expect_tx_warp(full_at + 8 * st, 0);
           bar = pm::dsmem_addr(tail + st, rank);
-          pm::mbar_arrive_expect_tx_warp(tail + st, bytes);
+          pm::mbar_arrive_expect_tx_warp(pm::smem_u32(tail + st), bytes);
         } else if (rank == 0) {
-          pm::mbar_arrive_expect_tx_warp(full + st, 2 * bytes);
+          pm::mbar_arrive_expect_tx_warp(full_at + 8 * st, 2 * bytes);
         }
-        if (MODE == kGradW) {
-          const int r0 = t.row0 + k0, n0 = t.m * 256 + rank * 128, c0 = t.n * 256 + rank * half;
-          if (a.a_chunks == 2) {
-            pm::tma2_load_4d_warp(sa, &tmA, 0, r0, n0 >> 6, 0, bar);
-          } else {
-            pm::tma2_load_4d_warp(sa, &tmA, n0, r0, 0, 0, bar);
-            pm::tma2_load_4d_warp(sa + kChunk, &tmA, n0 + 64, r0, 0, 0, bar);
-          }
-          if (a.b_chunks == 2 && half == 128) {
-            pm::tma2_load_4d_warp(sb, &tmB, 0, r0, c0 >> 6, 0, bar);
-          } else {
-            pm::tma2_load_2d_warp(sb, &tmB64, c0, r0, bar);
-            if (parts > 1) pm::tma2_load_2d_warp(sb + kChunk, &tmB64, c0 + 64, r0, bar);
-          }
-        } else {
-          const int f0 = t.m * 256 + rank * 128;
-          if (MODE == kForward && GATED) {  // 8 groups of 8 gate rows and the matching 8 up rows
-            pm::tma2_load_5d_warp(sa, &tmA, k0, 0, 0, f0 >> 4, t.e, bar);
-          } else if (MODE == kForward) {
-            pm::tma2_load_4d_warp(sa, &tmA, k0, f0, t.e, 0, bar);
-          } else {
-            if (a.a_chunks == 2) {
-              pm::tma2_load_4d_warp(sa, &tmA, 0, k0, f0 >> 6, t.e, bar);
-            } else {
-              pm::tma2_load_4d_warp(sa, &tmA, f0, k0, 0, t.e, bar);
-              pm::tma2_load_4d_warp(sa + kChunk, &tmA, f0 + 64, k0, 0, t.e, bar);
-            }
-          }
-          const int r0 = t.row0 + rank * half;
-          if (half > 96)
-            pm::tma2_load_2d_warp(sb, &tmB, k0, r0, bar);
-          else if (half > 32)
-            pm::tma2_load_2d_warp(sb, &tmB64, k0, r0, bar);
+        if (simple) {
+          if (MODE == kGradW)
+            pm::tma2_stage_55_warp(sa, &tmA, t.row0 + k0, f0 >> 6, sb, &tmB, c0 >> 6, bar);
+          else if (MODE == kGradX)
+            pm::tma2_stage_52_warp(sa, &tmA, 0, k0, f0 >> 6, t.e, 0, sb, mb, k0, r0, bar);
+          else if (GATED)  // 8 groups of 8 gate rows and the matching 8 up rows
+            pm::tma2_stage_52_warp(sa, &tmA, k0, 0, 0, f0 >> 4, t.e, sb, mb, k0, r0, bar);
           else
-            pm::tma2_load_2d_warp(sb, &tmB32, k0, r0, bar);
-          if (parts == 2) pm::tma2_load_2d_warp(sb + 64 * 128, &tmB32, k0, r0 + 64, bar);
+            pm::tma2_stage_52_warp(sa, &tmA, k0, f0, t.e, 0, 0, sb, mb, k0, r0, bar);
+        } else {  // MN-major operands whose chunks are no dimension: a load for each
+          const int y = MODE == kGradW ? t.row0 + k0 : k0, w = MODE == kGradW ? 0 : t.e;
+          if (a.a_chunks == 2) {
+            pm::tma2_load_5d_warp(sa, &tmA, 0, y, f0 >> 6, w, 0, bar);
+          } else {
+            pm::tma2_load_5d_warp(sa, &tmA, f0, y, 0, w, 0, bar);
+            pm::tma2_load_5d_warp(sa + kChunk, &tmA, f0 + 64, y, 0, w, 0, bar);
+          }
+          if (MODE == kGradX) {
+            pm::tma2_load_2d_warp(sb, mb, k0, r0, bar);
+          } else {
+            pm::tma2_load_2d_warp(sb, &tmB64, c0, y, bar);
+            if (parts == 2) pm::tma2_load_2d_warp(sb + kChunk, &tmB64, c0 + 64, y, bar);
+          }
         }
+        if (MODE != kGradW && parts == 2) pm::tma2_load_2d_warp(sb + 64 * 128, &tmB32, k0, r0 + 64, bar);
         if (issued < kStages) ++issued;
         if (++st == kStages) { st = 0; ph ^= 1; }
       }
@@ -266,28 +261,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const bool gone = stopped();
     for (int j = 1; j <= issued; ++j) {
       const int s = (st - j + kStages) % kStages;
-      pm::mbar_wait(empty + s, s < st ? ph : ph ^ 1, gone ? nullptr : site(), 406, gone ? 20000000ull : 2000000000ull);
+      pm::mbar_wait_warp(empty_at + 8 * s, s < st ? ph : ph ^ 1, gone ? nullptr : a.err, 406, gone ? 20000000ull : 2000000000ull);
     }
   } else if (warp == 1 && (rank == 0 || MODE == kGradW)) {
     // ------------------------------------------------------------------ MMA issuer (leader), ragged rows (both)
+    // stage 0's operands; 16 of the reduced dimension are 32 bytes of a K-major row, 16 rows of an MN-major chunk
+    constexpr int kAStep = MODE == kForward ? 2 : 128, kBStep = MODE == kGradW ? 128 : 2;
+    const uint64_t a0 = pm::make_sdesc(base, MODE == kForward ? 16 : kChunk, 1024);
+    const uint64_t b0 = pm::make_sdesc(base + C::kABytes, MODE == kGradW ? kChunk : 16, 1024);
     int st = 0, buf = 0;
     uint32_t ph = 0, dph = 0, tail_ph = 0;
     while (!stopped() && walk.next(t)) {
       if (t.nk == 0) continue;
       if (rank == 0) {
-        if (!agreed(pm::mbar_wait_cluster(d_empty + buf, dph ^ 1, site(), 402))) break;
+        if (!wait_cluster(pm::smem_u32(d_empty + buf), dph ^ 1, 402)) break;
         pm::tc_fence_after();
       }
       const uint32_t idesc = pm::make_idesc_f16(256, t.cols, a.half ? 0 : 1, MODE == kForward ? 0 : 1, MODE == kGradW ? 1 : 0);
       const uint32_t d = tmem + buf * 256;
       bool ok = true;
       for (int i = 0; i < t.nk && ok; ++i) {
-        if (rank == 0) ok = agreed(pm::mbar_wait(full + st, ph, site(), 403));
+        if (rank == 0) ok = wait(full_at + 8 * st, ph, 403);
         uint8_t* sp = smem + st * C::kStageBytes;
         int steps = 4;
         if (MODE == kGradW && ok && t.rows - i * kTileK < kTileK) {
           // steps of 16 rows, the last of them completed with zero rows (every column chunk of the stage)
-          ok = agreed(pm::mbar_wait(tail + st, (tail_ph >> st) & 1, site(), 407));
+          ok = wait(pm::smem_u32(tail + st), (tail_ph >> st) & 1, 407);
           const int have = t.rows - i * kTileK;
           steps = (have + 15) / 16;
           const int pad = steps * 16 - have, chunks = 2 + ((t.cols >> 1) + 63) / 64;
@@ -300,23 +299,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           if (rank == 1) {
             if (lane == 0) pm::mbar_arrive_cluster(pm::dsmem_addr(peer_tail + st, 0));
           } else if (ok) {
-            ok = agreed(pm::mbar_wait_cluster(peer_tail + st, (tail_ph >> st) & 1, site(), 408));
+            ok = wait_cluster(pm::smem_u32(peer_tail + st), (tail_ph >> st) & 1, 408);
           }
           tail_ph ^= 1u << st;
         }
         if (rank == 0 && ok) {
           pm::tc_fence_after();
-          const uint32_t sa = pm::smem_u32(sp), sb = sa + C::kABytes;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (MODE == kGradW && k >= steps) break;
-            const uint64_t bd = MODE == kGradW ? pm::make_sdesc(sb + k * 2048, kChunk, 1024)
-                                               : pm::make_sdesc(sb + 32 * k, 16, 1024);
-            const uint64_t ad = MODE == kForward ? pm::make_sdesc(sa + 32 * k, 16, 1024)
-                                                 : pm::make_sdesc(sa + k * 2048, kChunk, 1024);
-            pm::umma2_f16_warp(d, ad, bd, idesc, (i | k) ? 1u : 0u);
+          const uint64_t ad = a0 + st * (C::kStageBytes >> 4), bd = b0 + st * (C::kStageBytes >> 4);
+          if (MODE != kGradW || steps == 4) {
+            pm::umma2_f16_stage_warp<kAStep, kBStep>(d, ad, bd, idesc, i ? 1u : 0u, empty_at + 8 * st);
+          } else {
+            for (int k = 0; k < steps; ++k) pm::umma2_f16_warp(d, ad + k * kAStep, bd + k * kBStep, idesc, (i | k) ? 1u : 0u);
+            pm::umma2_commit_both_warp(empty + st);
           }
-          pm::umma2_commit_both_warp(empty + st);
         }
         if (++st == kStages) { st = 0; ph ^= 1; }
       }
@@ -327,7 +322,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     }
     if (rank == 0) {
       pm::umma2_commit_both_warp(drain);  // arrives once every MMA issued above has completed
-      pm::mbar_wait(drain, 0, site(), 404);
+      pm::mbar_wait_warp(pm::smem_u32(drain), 0, a.err, 404);
     }
   } else if (warp >= 2) {
     // ------------------------------------------------------------------ epilogue (warps 2-9 of both CTAs)
@@ -383,7 +378,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     while (!stopped() && walk.next(t)) {
       const bool zero = t.nk == 0;
       if (!zero) {
-        if (!agreed(pm::mbar_wait(d_full + buf, dph, site(), 405))) break;
+        if (!wait(pm::smem_u32(d_full + buf), dph, 405)) break;
         pm::tc_fence_after();
       }
       const uint32_t td = tmem + buf * 256 + ((uint32_t)(32 * q) << 16);
@@ -539,7 +534,7 @@ int launch_expert_mm(int mode, const ExpertMmCall& c, cudaStream_t stream) {
   const uint64_t K = c.K, N = c.N, E = c.E, P = c.P, I = N / 2;
   CUtensorMap ta, tb, tb64, tb32;  // A; B in boxes of 128, 64 and 32 rows (kGradW: two chunks, or one)
   const uint64_t dx[2] = {K, P}, sx[1] = {(uint64_t)c.xs * 2}, dd[2] = {N, P}, sd[1] = {(uint64_t)c.dzs * 2};
-  const uint64_t dw[4] = {K, N, E, 1}, sw[3] = {K * 2, N * K * 2, E * N * K * 2};
+  const uint64_t dw[5] = {K, N, E, 1, 1}, sw[4] = {K * 2, N * K * 2, 16, 16};
   // gated weights: [E][I / 8][gate | up][8][K]
   const uint64_t dg[5] = {K, 8, 2, I / 8, E}, sg[4] = {K * 2, I * K * 2, 8 * K * 2, N * K * 2};
   int rc;
@@ -548,10 +543,10 @@ int launch_expert_mm(int mode, const ExpertMmCall& c, cudaStream_t stream) {
   auto chunked = [&](CUtensorMap* m, const void* p, uint64_t width, uint64_t rows, uint64_t stride, uint64_t stack, int* n) {
     *n = width % 64 == 0 ? 2 : 1;
     const uint64_t wide = width / 64, whole = stack > 1 ? rows * stride : 16;
-    const uint64_t d2[4] = {64, rows, wide, stack}, s2[3] = {stride, 128, whole};
-    const uint64_t d1[4] = {width, rows, 1, stack}, s1[3] = {stride, 16, whole};
-    const uint32_t b2[4] = {64, kTileK, 2, 1}, b1[4] = {64, kTileK, 1, 1};
-    return *n == 2 ? make_tmap_16b_sw128(m, p, 4, d2, s2, b2, c.half) : make_tmap_16b_sw128(m, p, 4, d1, s1, b1, c.half);
+    const uint64_t d2[5] = {64, rows, wide, stack, 1}, s2[4] = {stride, 128, whole, 16};
+    const uint64_t d1[5] = {width, rows, 1, stack, 1}, s1[4] = {stride, 16, whole, 16};
+    const uint32_t b2[5] = {64, kTileK, 2, 1, 1}, b1[5] = {64, kTileK, 1, 1, 1};
+    return *n == 2 ? make_tmap_16b_sw128(m, p, 5, d2, s2, b2, c.half) : make_tmap_16b_sw128(m, p, 5, d1, s1, b1, c.half);
   };
   if (mode == kGradW) {
     const uint32_t box[2] = {64, kTileK};
@@ -576,8 +571,8 @@ int launch_expert_mm(int mode, const ExpertMmCall& c, cudaStream_t stream) {
     } else if (mode == kGradX) {
       if (!rc) rc = chunked(&ta, c.w, K, N, K * 2, E, &a.a_chunks);
     } else {
-      const uint32_t box[4] = {64, 128u, 1, 1};
-      if (!rc) rc = make_tmap_16b_sw128(&ta, c.w, 4, dw, sw, box, c.half);
+      const uint32_t box[5] = {kTileK, 128, 1, 1, 1};
+      if (!rc) rc = make_tmap_16b_sw128(&ta, c.w, 5, dw, sw, box, c.half);
     }
     a.N = (int)(mode == kForward ? N : K);
     a.nk = ceil_div(mode == kForward ? K : N, kTileK);
