@@ -68,11 +68,13 @@ __device__ __forceinline__ void tile_table(const ExpertMmArgs& a, int32_t* off, 
 //     memory.  Gated: A takes gate and up rows by turns, 8 and 8, so that a feature's two products lie 8 TMEM
 //     lanes apart and meet by one exchange within the warp.
 //   kGradW: A is dz^T (256 of n), B x^T (256 of k), both MN-major, reduced over the expert's rows.  The last
-//     stage reads into the next expert's rows, and 0 x NaN is NaN: each CTA zeroes those rows of both its
-//     operands in shared memory before the MMA.
+//     stage reads into the next expert's rows, and 0 x NaN is NaN: a warp of each CTA zeroes those rows of both
+//     its operands in shared memory, ahead of the MMA.
 //   kGradX reads W along its other dimension by an MN-major descriptor: nothing is transposed in memory.
-constexpr int kPairThreads = 320;  // warp 0 TMA producer, 1 MMA issuer (leader) / tail rows, 2-9 epilogue
 constexpr int kEpiWarps = 8;
+constexpr int kTrimWarp = 2 + kEpiWarps;
+// warp 0 TMA producer, 1 MMA issuer (leader), 2-9 epilogue, kGradW: 10 ragged rows
+constexpr int pair_threads(int mode) { return 32 * (kTrimWarp + (mode == kGradW ? 1 : 0)); }
 constexpr uint32_t kEpiWarpBytes = 32 * 64;  // staging of an epilogue warp: 32 rows x 32 columns
 constexpr uint32_t kHalf = 128 * 128;    // 128 rows x 64 elements: one CTA's A rows, or its half of B
 constexpr uint32_t kChunk = 64 * 128;    // MN-major operands: 64 reduced rows x 64 columns
@@ -135,7 +137,7 @@ struct PairWalker {
 };
 
 template <typename T, int MODE, bool GATED>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 1)
     expert_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                        const __grid_constant__ CUtensorMap tmB64, const __grid_constant__ CUtensorMap tmB32,
                        const ExpertMmArgs a) {
@@ -146,8 +148,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);  // leader's: both CTAs' loads of a stage
   uint64_t* empty = full + kMaxStages;       // each CTA's: the MMA has read its stage
   uint64_t* tail = empty + kMaxStages;       // kGradW, each CTA's: loads of an expert's ragged last stage
-  uint64_t* peer_tail = tail + kMaxStages;   // leader's: the peer has zeroed its ragged rows
-  uint64_t* d_full = peer_tail + kMaxStages; // [2], each CTA's
+  uint64_t* trimmed = tail + kMaxStages;     // leader's: both CTAs have zeroed the rows past the expert's last
+  uint64_t* d_full = trimmed + kMaxStages;   // [2], each CTA's
   uint64_t* d_empty = d_full + 2;            // [2], leader's: epilogue warps of both CTAs
   uint64_t* drain = d_empty + 2;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -166,7 +168,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       pm::mbar_init(full + s, 1);
       pm::mbar_init(empty + s, 1);
       pm::mbar_init(tail + s, 1);
-      pm::mbar_init(peer_tail + s, 1);
+      pm::mbar_init(trimmed + s, 2);
     }
     for (int s = 0; s < 2; ++s) {
       pm::mbar_init(d_full + s, 1);
@@ -263,68 +265,72 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const int s = (st - j + kStages) % kStages;
       pm::mbar_wait_warp(empty_at + 8 * s, s < st ? ph : ph ^ 1, gone ? nullptr : a.err, 406, gone ? 20000000ull : 2000000000ull);
     }
-  } else if (warp == 1 && (rank == 0 || MODE == kGradW)) {
-    // ------------------------------------------------------------------ MMA issuer (leader), ragged rows (both)
+  } else if (warp == 1 && rank == 0) {
+    // ------------------------------------------------------------------ MMA issuer (leader)
     // stage 0's operands; 16 of the reduced dimension are 32 bytes of a K-major row, 16 rows of an MN-major chunk
     constexpr int kAStep = MODE == kForward ? 2 : 128, kBStep = MODE == kGradW ? 128 : 2;
     const uint64_t a0 = pm::make_sdesc(base, MODE == kForward ? 16 : kChunk, 1024);
     const uint64_t b0 = pm::make_sdesc(base + C::kABytes, MODE == kGradW ? kChunk : 16, 1024);
     int st = 0, buf = 0;
-    uint32_t ph = 0, dph = 0, tail_ph = 0;
+    uint32_t ph = 0, dph = 0, trim_ph = 0;
     while (!stopped() && walk.next(t)) {
       if (t.nk == 0) continue;
-      if (rank == 0) {
-        if (!wait_cluster(pm::smem_u32(d_empty + buf), dph ^ 1, 402)) break;
-        pm::tc_fence_after();
-      }
+      if (!wait_cluster(pm::smem_u32(d_empty + buf), dph ^ 1, 402)) break;
+      pm::tc_fence_after();
       const uint32_t idesc = pm::make_idesc_f16(256, t.cols, a.half ? 0 : 1, MODE == kForward ? 0 : 1, MODE == kGradW ? 1 : 0);
       const uint32_t d = tmem + buf * 256;
       bool ok = true;
-      for (int i = 0; i < t.nk && ok; ++i) {
-        if (rank == 0) ok = wait(full_at + 8 * st, ph, 403);
-        uint8_t* sp = smem + st * C::kStageBytes;
-        int steps = 4;
-        if (MODE == kGradW && ok && t.rows - i * kTileK < kTileK) {
-          // steps of 16 rows, the last of them completed with zero rows (every column chunk of the stage)
-          ok = wait(pm::smem_u32(tail + st), (tail_ph >> st) & 1, 407);
-          const int have = t.rows - i * kTileK;
-          steps = (have + 15) / 16;
-          const int pad = steps * 16 - have, chunks = 2 + ((t.cols >> 1) + 63) / 64;
-          for (int j = lane; j < pad * chunks * 8; j += 32) {
-            const int chunk = j / (pad * 8), in = j - chunk * pad * 8, r = have + in / 8;
-            *reinterpret_cast<uint4*>(sp + chunk * kChunk + r * 128 + (in & 7) * 16) = make_uint4(0, 0, 0, 0);
-          }
-          pm::fence_proxy_async_smem();
-          __syncwarp();
-          if (rank == 1) {
-            if (lane == 0) pm::mbar_arrive_cluster(pm::dsmem_addr(peer_tail + st, 0));
-          } else if (ok) {
-            ok = wait_cluster(pm::smem_u32(peer_tail + st), (tail_ph >> st) & 1, 408);
-          }
-          tail_ph ^= 1u << st;
-        }
-        if (rank == 0 && ok) {
+      for (int i = 0; i < t.nk; ++i) {
+        const uint64_t ad = a0 + st * (C::kStageBytes >> 4), bd = b0 + st * (C::kStageBytes >> 4);
+        const int have = t.rows - i * kTileK;
+        if (MODE == kGradW && have < kTileK) {  // the ragged stage is ready when both CTAs have zeroed its rows
+          ok = wait_cluster(pm::smem_u32(trimmed + st), (trim_ph >> st) & 1, 403);
+          if (!ok) break;
+          trim_ph ^= 1u << st;
           pm::tc_fence_after();
-          const uint64_t ad = a0 + st * (C::kStageBytes >> 4), bd = b0 + st * (C::kStageBytes >> 4);
-          if (MODE != kGradW || steps == 4) {
-            pm::umma2_f16_stage_warp<kAStep, kBStep>(d, ad, bd, idesc, i ? 1u : 0u, empty_at + 8 * st);
-          } else {
-            for (int k = 0; k < steps; ++k) pm::umma2_f16_warp(d, ad + k * kAStep, bd + k * kBStep, idesc, (i | k) ? 1u : 0u);
-            pm::umma2_commit_both_warp(empty + st);
-          }
+          for (int k = 0; k < (have + 15) / 16; ++k)
+            pm::umma2_f16_warp(d, ad + k * kAStep, bd + k * kBStep, idesc, (i | k) ? 1u : 0u);
+          pm::umma2_commit_both_warp(empty + st);
+        } else {
+          ok = wait(full_at + 8 * st, ph, 404);
+          if (!ok) break;
+          pm::tc_fence_after();
+          pm::umma2_f16_stage_warp<kAStep, kBStep>(d, ad, bd, idesc, i ? 1u : 0u, empty_at + 8 * st);
         }
         if (++st == kStages) { st = 0; ph ^= 1; }
       }
       if (!ok) break;
-      if (rank == 0) pm::umma2_commit_both_warp(d_full + buf);
+      pm::umma2_commit_both_warp(d_full + buf);
       buf ^= 1;
       if (buf == 0) dph ^= 1;
     }
-    if (rank == 0) {
-      pm::umma2_commit_both_warp(drain);  // arrives once every MMA issued above has completed
-      pm::mbar_wait_warp(pm::smem_u32(drain), 0, a.err, 404);
+    pm::umma2_commit_both_warp(drain);  // arrives once every MMA issued above has completed
+    pm::mbar_wait_warp(pm::smem_u32(drain), 0, a.err, 407);
+  } else if (MODE == kGradW && warp == kTrimWarp) {
+    // ------------------------------------------------------------------ ragged rows (both CTAs)
+    // The MMA takes steps of 16 rows: the last one of an expert is completed with zero rows in every column chunk
+    // (4 chunks of 8 16-byte units: a lane each).
+    const uint32_t trimmed_leader = pm::dsmem_addr(trimmed, 0);
+    int st = 0;
+    uint32_t ph = 0;
+    while (!stopped() && walk.next(t)) {
+      if (t.nk == 0) continue;
+      st = (st + t.nk - 1) % kStages;
+      const int have = t.rows - (t.nk - 1) * kTileK;
+      if (have < kTileK) {
+        if (!wait(pm::smem_u32(tail + st), (ph >> st) & 1, 408)) break;
+        ph ^= 1u << st;
+        if ((lane >> 3) < 2 + ((t.cols >> 1) + 63) / 64) {
+          uint8_t* at = smem + st * C::kStageBytes + (lane >> 3) * kChunk + (lane & 7) * 16;
+          for (int r = have; r & 15; ++r) *reinterpret_cast<uint4*>(at + r * 128) = make_uint4(0, 0, 0, 0);
+        }
+        pm::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) pm::mbar_arrive_cluster(trimmed_leader + 8 * st);
+      }
+      if (++st == kStages) st = 0;
     }
-  } else if (warp >= 2) {
+  } else if (warp >= 2 && warp < 2 + kEpiWarps) {
     // ------------------------------------------------------------------ epilogue (warps 2-9 of both CTAs)
     const int q = warp & 3, side = (warp - 2) >> 2;  // TMEM lane quadrant; half of the columns
     uint8_t* stage = smem + C::kEpiOff + (warp - 2) * kEpiWarpBytes;
@@ -503,7 +509,7 @@ int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap&
   if (smem > kMaxSmem) return -2;
   auto* fn = expert_pair_kernel<T, MODE, GATED>;
   cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  fn<<<a.num_sms / 2 * 2, kPairThreads, smem, stream>>>(ta, tb, tb64, tb32, a);
+  fn<<<a.num_sms / 2 * 2, pair_threads(MODE), smem, stream>>>(ta, tb, tb64, tb32, a);
   return 0;
 }
 template <typename T>
