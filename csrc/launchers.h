@@ -289,6 +289,8 @@ struct NormBwdArgs {
 };
 int rmsnorm_bwd_slots(int64_t rows, int n, bool res, int num_sms);
 void launch_rmsnorm_bwd(const NormBwdArgs& a, int slots, cudaStream_t stream);
+// n codes (contiguous, a multiple of 32) with their scale bytes -> BF16.
+void launch_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t n, void* out, cudaStream_t stream);
 
 // Token rows sorted by expert and back (csrc/expert_dispatch.cu).
 int launch_expert_order(const void* ids, bool wide, int64_t n, int64_t base, int E, int32_t* offsets, int32_t* slots,

@@ -295,6 +295,26 @@ __global__ void __launch_bounds__(256) norm_dw_kernel(const float* __restrict__ 
   if (threadIdx.y == 0 && c < n) *reinterpret_cast<float4*>(dw + c) = s;
 }
 
+// code x 2^(scale - 127) in BF16 (exact: an E4M3 value has four significant bits).  Thread per 16 codes; memory bound.
+__global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint4* __restrict__ codes,
+                                                            const uint8_t* __restrict__ scales, int64_t n16,
+                                                            uint4* __restrict__ out) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n16) return;
+  const uint4 c = codes[i];
+  const float s = exp2f((float)scales[i >> 1] - 127.f);
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  uint32_t o[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 lo = __half22float2(pm::e4m3x2_to_h2((uint16_t)w[j])), hi = __half22float2(pm::e4m3x2_to_h2((uint16_t)(w[j] >> 16)));
+    o[2 * j] = rows::pack2<__nv_bfloat16>(lo.x * s, lo.y * s);
+    o[2 * j + 1] = rows::pack2<__nv_bfloat16>(hi.x * s, hi.y * s);
+  }
+  out[2 * i] = make_uint4(o[0], o[1], o[2], o[3]);
+  out[2 * i + 1] = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
 // Threads of a row for `vpt` vectors each (a power of two from 4 to 32, or whole warps), and the rows of a
 // block of about 256 threads.
 dim3 norm_block(int n, int vpt) {
@@ -363,4 +383,10 @@ void launch_rmsnorm_bwd(const NormBwdArgs& a, int slots, cudaStream_t stream) {
     fn<<<slots / block.y, block, p.smem, stream>>>(a, p.stages);
   }
   norm_dw_kernel<<<(a.n + 15) / 16, dim3(4, 64), 0, stream>>>(a.part, slots, a.n, a.dw);
+}
+
+void launch_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t n, void* out, cudaStream_t stream) {
+  if (n == 0) return;
+  mx_dequantize_kernel<<<(unsigned)((n / 16 + 255) / 256), 256, 0, stream>>>(reinterpret_cast<const uint4*>(codes), scales,
+                                                                           n / 16, static_cast<uint4*>(out));
 }

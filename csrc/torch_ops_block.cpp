@@ -149,6 +149,19 @@ std::tuple<Tensor, Tensor, OptTensor> rmsnorm_backward(const Tensor& dh_in, cons
   return {dx, dw, dxf};
 }
 
+Tensor mx_dequantize(const Tensor& codes_in, const Tensor& scales_in) {
+  const Tensor codes = codes_in.contiguous(), scales = scales_in.contiguous();
+  TORCH_CHECK(codes.is_cuda() && codes.dim() == 2 && codes.scalar_type() == torch::kUInt8 && codes.size(1) % 32 == 0,
+              "mx_dequantize: codes must be a CUDA uint8 [rows, n] tensor, n a multiple of 32");
+  check_rows(codes, scales, codes.size(0), codes.size(1) / 32, torch::kUInt8, "scales");
+  TORCH_CHECK(codes.numel() == 0 || on16(codes), "mx_dequantize: codes must start on a 16-byte boundary");
+  const c10::cuda::CUDAGuard g(codes.device());
+  Tensor out = make({codes.size(0), codes.size(1)}, codes, torch::kBFloat16);
+  launch_mx_dequantize(codes.data_ptr<uint8_t>(), scales.data_ptr<uint8_t>(), codes.numel(), out.data_ptr(), stream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return out;
+}
+
 // -> (offsets [E + 1], slots [T, k], pairs [T k])
 std::tuple<Tensor, Tensor, Tensor> expert_order(const Tensor& ids_in, int64_t num_experts, int64_t expert_base) {
   const Tensor ids = ids_in.contiguous();
@@ -527,6 +540,7 @@ void bind_block_ops(pybind11::module_& m) {
   const auto unlocked = pybind11::call_guard<pybind11::gil_scoped_release>();
   m.def("add_rmsnorm_mx", &add_rmsnorm_mx_op, "residual add + RMSNorm -> MXFP8 rows", unlocked);
   m.def("rmsnorm_backward", &rmsnorm_backward, "gradient of residual add + RMSNorm", unlocked);
+  m.def("mx_dequantize", &mx_dequantize, "MXFP8 rows -> BF16 (exact)", unlocked);
   m.def("expert_order", &expert_order, "stable sort of (token, choice) pairs by expert", unlocked);
   m.def("expert_gather", &gather_op, "token rows -> rows sorted by expert", unlocked);
   m.def("expert_gather_mx", &expert_gather, "MXFP8 token rows -> rows sorted by expert", unlocked);

@@ -168,7 +168,8 @@ class EngineConfig:
     device: str = "cuda"
     fused_collectives: bool = True
     # MoE activation precision, as the reference's --flashinfer-mxfp4-moe-precision: "default" quantizes
-    # expert inputs to MXFP8 (E4M3 + UE8M0 per 32) on sm_100, "bf16" keeps them in BF16.
+    # expert inputs to MXFP8 (E4M3 + UE8M0 per 32) on sm_100, "bf16" keeps them in BF16; "grouped" (BF16
+    # experts only) runs every expert's products in one launch instead of an expert at a time.
     moe_precision: str = "default"
     # C4 attention over Packed KV: "direct" reads the planes inside the attention kernel; "adapter"
     # first reconstructs the selected rows as Native records (the reference's Adapter mode)
@@ -215,8 +216,8 @@ class EngineConfig:
             raise ValueError("prefix_block_tokens must be a multiple of 256")
         if self.hicache_ratio <= 0:
             raise ValueError("hicache_ratio must be positive")
-        if self.moe_precision not in ("default", "bf16"):
-            raise ValueError("moe_precision must be 'default' or 'bf16'")
+        if self.moe_precision not in ("default", "bf16", "grouped"):
+            raise ValueError("moe_precision must be 'default', 'bf16' or 'grouped'")
         if self.decode_impl not in ("direct", "adapter"):
             raise ValueError("decode_impl must be 'direct' or 'adapter'")
         if self.decode_impl == "adapter" and self.kv_cache_format != "direct":

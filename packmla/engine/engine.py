@@ -237,6 +237,8 @@ class Engine:
               comm=None, max_context: int = 1 << 15, max_requests: int | None = None, kv_bytes: int | None = None,
               seed: int = 0, weights: dict | None = None) -> "Engine":
         engine_cfg.validate()
+        if engine_cfg.moe_precision == "grouped" and model_cfg.expert_format == "mxfp4":
+            raise ValueError("moe_precision 'grouped' needs BF16 experts")
         dev = torch.device(device)
         W = weights if weights is not None else init_weights(model_cfg, rank, world, dev, seed,
                                                              dp_attention=engine_cfg.dp_attention)

@@ -23,7 +23,8 @@ def decode_uses_partials(splits: int) -> bool:
 # kernels launched per extension entry point (for the bench's launch count): a number, or a function of
 # the call's positional arguments
 KERNELS_PER_CALL = {"native_store": 1, "packed_store": 1,
-                    "sparse_mla_decode": lambda a: 2 if decode_uses_partials(int(a[16])) else 1, "moe_fp4": 3, "moe_fp4_mma": 4, "add_rmsnorm": 1, "bs_probe": 1, "moe_mxf4": 4, "bs_probe2": 1, "rope_q": 1, "comp_pool": 1, "route_topk": 1, "silu_mul": 1, "index_key_store": 1, "index_select": 2, "umma_probe": 1, "gemm_allreduce": 1, "allreduce": 1}
+                    "sparse_mla_decode": lambda a: 2 if decode_uses_partials(int(a[16])) else 1, "moe_fp4": 3, "moe_fp4_mma": 4, "add_rmsnorm": 1, "bs_probe": 1, "moe_mxf4": 4, "bs_probe2": 1, "rope_q": 1, "comp_pool": 1, "route_topk": 1, "silu_mul": 1, "index_key_store": 1, "index_select": 2, "umma_probe": 1, "gemm_allreduce": 1, "allreduce": 1,
+                    "rmsnorm_backward": 2, "expert_linear_backward": lambda a: int(a[4]) + int(a[5])}
 
 
 class _Counting:

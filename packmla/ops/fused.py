@@ -105,7 +105,7 @@ def _norm_oracle(s: torch.Tensor, w: torch.Tensor, eps: float):
 
 
 def mx_quantize(h: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """fp32 rows [T, n] -> (E4M3 codes [T, n], UE8M0 scale bytes [T, n / 32]), uint8 (the rule of `mx_dequantize`'s inverse)."""
+    """fp32 rows [T, n] -> (E4M3 codes [T, n], UE8M0 scale bytes [T, n / 32]), uint8: the rule of `add_rmsnorm_mx`."""
     b = h.float().unflatten(-1, (h.shape[1] // MX_GROUP, MX_GROUP))
     e = codec.ue8m0_exponent(b.abs().amax(-1))
     return codec.e4m3_encode(b * codec.exp2_int(-e)[..., None]).reshape(h.shape), (e + 127).to(torch.uint8)
@@ -113,6 +113,8 @@ def mx_quantize(h: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """MXFP8 rows -> code x 2^(scale - 127).  Exact in BF16 and fp32 (E4M3 has four significant bits)."""
+    if codes.is_cuda and dtype == torch.bfloat16:
+        return ext().mx_dequantize(codes, scales)
     v = codec.e4m3_decode(codes).unflatten(-1, (codes.shape[1] // MX_GROUP, MX_GROUP))
     return (v * codec.exp2_int(scales.to(torch.int32) - 127)[..., None]).reshape(codes.shape).to(dtype)
 

@@ -11,13 +11,15 @@ all-reduce combines ranks (the MoE down-projection partial sums).
   weight stream dequantized straight into register MMA fragments, gate/up with SiLU, down with the
   routed-weight scatter-add; weights use the fragment-ordered layout made once by
   `prepare_experts`.
-* BF16 experts (tiny CPU configs, tests): PyTorch reference.
+* BF16 experts (tiny CPU configs, tests): PyTorch reference; with precision "grouped" all experts' products
+  run in one launch each on rows sorted by expert (`experts_grouped`), differentiable.
 """
 from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
 
+from . import dispatch, grouped
 from ._ext import error_word, ext
 
 
@@ -46,6 +48,16 @@ def experts_reference(h, topk_ids, topk_w, w13, w2, expert_base, local_experts):
         y = (act @ w2[le].T).float()
         out.index_add_(0, tok, y * topk_w[tok, kk][:, None])
     return out
+
+
+def experts_grouped(h, topk_ids, topk_w, w13, w2, expert_base, local_experts):
+    """BF16 or FP16 experts -> fp32 [T, H]: tokens sorted by expert, gate/up products with SwiGLU and down
+    products of every expert in one launch each, weighted sum per token.  Nothing waits for the host.
+    Differentiable in h, topk_w, w13 and w2; the intermediate rows are rounded to h's type."""
+    order = dispatch.expert_order(topk_ids, local_experts, expert_base)
+    act = grouped.expert_linear(dispatch.gather(h, order), w13, order.offsets, activation="swiglu")
+    y = grouped.expert_linear(act, w2, order.offsets)
+    return dispatch.combine(y, order, topk_w, out_dtype=torch.float32)
 
 
 def fp4_dequant(w: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
@@ -233,8 +245,13 @@ def experts(h, topk_ids, topk_w, lw, expert_base, local_experts, expert_format, 
     """Routed experts -> fp32 [T, H] (sum over this rank's experts of w_k * expert_k(h)).
 
     precision "default": MXFP8 activations (tcgen05 block-scaled kernel, csrc/moe_mxf4.cu);
-    "bf16": BF16 activations (csrc/moe_fp4_mma.cu).  BF16 experts (tiny configs) use PyTorch.
+    "bf16": BF16 activations (csrc/moe_fp4_mma.cu).  BF16 experts (tiny configs) use PyTorch, or with precision
+    "grouped" the products of csrc/expert_mm.cu.
     """
+    if precision == "grouped":
+        if expert_format == "mxfp4":
+            raise ValueError("moe precision 'grouped' needs BF16 experts")
+        return experts_grouped(h, topk_ids, topk_w, lw["w13"], lw["w2"], expert_base, local_experts)
     if expert_format != "mxfp4":
         return experts_reference(h, topk_ids, topk_w, lw["w13"], lw["w2"], expert_base, local_experts)
     if precision not in ("default", "bf16"):

@@ -14,6 +14,9 @@ Within one layer call:
   3. owner runs its experts on the rows it received (unweighted outputs);
   4. outputs (bf16 by default) -> back to the source ranks (all-to-all), weighted and summed in fp32 per
      token in routing order.
+
+`forward_mx` is the same call on the MXFP8 rows of `ops.fused.add_rmsnorm_mx`: codes and scales cross the link
+(33 bytes per 32 values instead of 64), sorted by owner, gathered and summed by packmla's own kernels.
 """
 from __future__ import annotations
 
@@ -21,6 +24,8 @@ from typing import Callable
 
 import torch
 import torch.distributed as dist
+
+from ..ops import dispatch, fused
 
 
 class EPMoE:
@@ -70,6 +75,33 @@ class EPMoE:
         out = (pairs.view(T, k, -1) * topk_w.float()[..., None]).sum(1)
         self.last_counts = {"sent": send, "received": recv}
         return out
+
+    def forward_mx(self, codes: torch.Tensor, scales: torch.Tensor, topk_ids: torch.Tensor, topk_w: torch.Tensor,
+                   local_fn: Callable[[torch.Tensor, torch.Tensor], torch.Tensor],
+                   residual: torch.Tensor | None = None) -> torch.Tensor:
+        """`forward` of this rank's tokens as MXFP8 rows (codes [T, H], scale bytes [T, H / 32], uint8) ->
+        fp32 [T, H] = residual + sum_k w_k expert_k(row).  `local_fn` gets the values the rows stand for in BF16,
+        which holds them exactly: experts that quantize their inputs by the same rule (moe precision "default")
+        find the same codes.  A pair whose expert id is negative (a masked token) is not sent and adds nothing."""
+        T, k = topk_ids.shape
+        masked = topk_ids < 0
+        owner = torch.where(masked, -1, topk_ids // self.local_experts)
+        order = dispatch.expert_order(owner, self.world)
+        send_counts = (order.offsets[1:] - order.offsets[:-1]).long()
+        recv_counts = self._exchange(send_counts, self.world, [1] * self.world, [1] * self.world)
+        send, recv = send_counts.tolist(), recv_counts.tolist()
+        sent = sum(send)
+        rows, row_scales = dispatch.gather_mx(codes, scales, order)
+        pair = order.pairs[:sent].long()
+        local_ids = topk_ids.reshape(-1)[pair].long() % self.local_experts
+        r_codes = self._exchange(rows[:sent], sum(recv), send, recv)
+        r_scales = self._exchange(row_scales[:sent], sum(recv), send, recv)
+        r_ids = self._exchange(local_ids, sum(recv), send, recv)
+        y = local_fn(fused.mx_dequantize(r_codes, r_scales), r_ids).to(self.combine_dtype)
+        back = torch.zeros(T * k, y.shape[1], dtype=y.dtype, device=y.device)
+        back[:sent] = self._exchange(y, sent, recv, send)
+        self.last_counts = {"sent": send, "received": recv}
+        return dispatch.combine(back, order, topk_w.float(), residual, torch.float32)
 
 
 def local_expert_fn(lw: dict, expert_base: int, local_experts: int, expert_format: str,

@@ -49,7 +49,7 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--disable-cuda-graph", action="store_true")
     ap.add_argument("--enable-hierarchical-cache", action="store_true")
     ap.add_argument("--hicache-ratio", type=float, default=2.0)
-    ap.add_argument("--moe-precision", default="default", choices=["default", "bf16"])
+    ap.add_argument("--moe-precision", default="default", choices=["default", "bf16", "grouped"])
     ap.add_argument("--decode-impl", default="direct", choices=["direct", "adapter"])
     ap.add_argument("--collectives", default="fused", choices=["fused", "nccl"])
     ap.add_argument("--seed", "--random-seed", dest="seed", type=int, default=0)

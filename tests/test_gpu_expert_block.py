@@ -531,3 +531,50 @@ def test_products_refusals(cuda):
     assert grouped.expert_linear(x[:0], w, spread([0, 0])).shape == (0, 32)
     dx, dw = grouped.expert_linear_backward(torch.zeros(0, 32, device="cuda", dtype=BF16), x[:0], w, spread([0, 0]))
     assert dx.shape == (0, 64) and (dw == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------ paths
+@pytest.mark.parametrize("rows,n", [(1, 32), (7, 96), (300, 4096), (0, 64)])
+def test_mx_dequantize_is_exact(cuda, rows, n):
+    codes = torch.randint(0, 256, (rows, n), device="cuda", dtype=torch.uint8)
+    codes[codes & 127 == 127] = 0  # no NaN codes
+    scales = torch.randint(100, 150, (rows, n // 32), device="cuda", dtype=torch.uint8)
+    got = fused.mx_dequantize(codes, scales)
+    assert got.dtype == BF16
+    assert torch.equal(got.cpu(), fused.mx_dequantize(codes.cpu(), scales.cpu()))
+
+
+def test_grouped_experts_match_the_expert_loop(cuda):
+    from packmla.ops import moe
+
+    g = gen(11)
+    T, k, E, H, I = 130, 3, 12, 256, 192
+    h = randn(g, T, H, dtype=BF16)
+    lw = {"w13": randn(g, E, 2 * I, H, dtype=BF16, scale=H ** -0.5), "w2": randn(g, E, H, I, dtype=BF16, scale=I ** -0.5)}
+    ids = torch.rand(T, 2 * E, device="cuda", generator=g).topk(k).indices.int()  # half of them on other ranks
+    w = torch.rand(T, k, device="cuda", generator=g)
+    ref_out = moe.experts(h, ids, w, lw, 0, E, "bf16")
+    got = moe.experts(h, ids, w, lw, 0, E, "bf16", precision="grouped")
+    check_errors(cuda)
+    assert (got - ref_out).norm() <= 2 ** -7 * ref_out.norm()
+
+
+def test_block_on_the_gpu_matches_the_cpu(cuda):
+    from packmla.training.expert_block import ExpertBlock, fit
+
+    dev = ExpertBlock(128, 64, 8, 2, device="cuda", seed=1)
+    cpu = ExpertBlock(128, 64, 8, 2, device="cpu", seed=1)
+    for a, b in zip(cpu.parameters(), dev.parameters()):
+        a.data.copy_(b.data)
+    g = torch.Generator().manual_seed(5)
+    x, d, v = (torch.randn(70, 128, generator=g).bfloat16() for _ in range(3))
+    grads = []
+    for block, where in ((dev, "cuda"), (cpu, "cpu")):
+        xr = x.to(where).requires_grad_(True)
+        stream, out = block(xr, d.to(where), (torch.arange(70) % 9 != 0).to(where))
+        grads.append([t.cpu().double() for t in (out.detach(), *torch.autograd.grad(out, [xr, *block.parameters()], v.to(where)))])
+    check_errors(cuda)
+    for a, b in zip(*grads):  # both sides round BF16 rows at the same places; sums differ in order
+        assert (a - b).norm() <= 2e-2 * b.norm()
+    r = fit(tokens=512, hidden=128, inter=64, experts=8, topk=2, steps=30, lr=3e-3, device="cuda")
+    assert r["last_loss"] < 0.9 * r["first_loss"]
