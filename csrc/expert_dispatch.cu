@@ -307,12 +307,13 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const CombineArgs a
   }
 }
 
-// Block per token: dout's columns are read once, every choice's y row once; the k dot products end in one
-// block reduction per batch of choices.
+// Block per token, the last token first: the rows that the forward pass read last may still be in L2.  dout's
+// columns are read once, every choice's y row once; the k dot products end in one block reduction per batch of
+// choices.
 template <typename T, typename O, int NV>
 __global__ void __launch_bounds__(256) expert_combine_bwd_kernel(const CombineBwdArgs a) {
   __shared__ float red[kBatch][8];
-  const int64_t t = blockIdx.x;
+  const int64_t t = (int64_t)gridDim.x - 1 - blockIdx.x;
   const int nv = a.width / NV, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int32_t* slot = a.slots + t * a.k;
   const float* wt = a.weights + t * a.ws;
@@ -445,7 +446,7 @@ int launch_expert_order(const void* ids, bool wide, int64_t n, int64_t base, int
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   auto go = [&](auto* fn, auto* p) {
-    cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (smem > 48 * 1024) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (cluster > 8) cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     return (int)cudaLaunchKernelEx(&cfg, fn, p, (int)n, base, E, offsets, slots, pairs);
   };

@@ -469,34 +469,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
 
 // ----------------------------------------------------------------------------- SwiGLU gradient
 // da = gradient of silu(g) u; z = [g | u] rows: dg = da u s (1 + g (1 - s)), du = da g s with s = sigmoid(g).
-// Rows past offsets[E] are zero.  Memory bound: 6 bytes read and 4 written per value of da.
+// Rows past offsets[E] are zero.  Memory bound: 6 bytes read and 4 written per value of da; a block per row (58 us
+// for 16384 x 2048, 5.8 TB/s; walking blocks 61 us).
 template <typename T>
 __global__ void __launch_bounds__(256) swiglu_bwd_kernel(const T* __restrict__ da, int64_t das,
                                                          const T* __restrict__ z, int64_t zs, T* __restrict__ dz,
                                                          int64_t P, int I, const int32_t* __restrict__ offsets, int E) {
   const int nv = I / 8;
   const int64_t total = offsets[E];
-  for (int64_t row = blockIdx.x; row < P; row += gridDim.x) {
-    for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < nv; c += gridDim.y * blockDim.x) {
-      float d[8], g[8], u[8];
-      if (row < total) {
-        rows::load8<T>(da + row * das + c * 8, d);
-        rows::load8<T>(z + row * zs + c * 8, g);
-        rows::load8<T>(z + row * zs + I + c * 8, u);
+  const int64_t row = blockIdx.x;
+  for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < nv; c += gridDim.y * blockDim.x) {
+    float d[8], g[8], u[8];
+    if (row < total) {
+      rows::load8<T>(da + row * das + c * 8, d);
+      rows::load8<T>(z + row * zs + c * 8, g);
+      rows::load8<T>(z + row * zs + I + c * 8, u);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float s = 1.f / (1.f + __expf(-g[i])), gs = g[i] * s;
-          const float up = u[i];
-          u[i] = d[i] * gs;
-          g[i] = d[i] * up * (s + gs * (1.f - s));
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = u[i] = 0.f;
+      for (int i = 0; i < 8; ++i) {
+        const float s = 1.f / (1.f + __expf(-g[i])), gs = g[i] * s;
+        const float up = u[i];
+        u[i] = d[i] * gs;
+        g[i] = d[i] * up * (s + gs * (1.f - s));
       }
-      *reinterpret_cast<uint4*>(dz + row * 2 * I + c * 8) = rows::pack8<T>(g);
-      *reinterpret_cast<uint4*>(dz + row * 2 * I + I + c * 8) = rows::pack8<T>(u);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g[i] = u[i] = 0.f;
     }
+    *reinterpret_cast<uint4*>(dz + row * 2 * I + c * 8) = rows::pack8<T>(g);
+    *reinterpret_cast<uint4*>(dz + row * 2 * I + I + c * 8) = rows::pack8<T>(u);
   }
 }
 
@@ -594,8 +594,7 @@ void launch_swiglu_bwd(const void* da, int64_t das, const void* z, int64_t zs, v
                        const int32_t* offsets, int E, int half, int num_sms, cudaStream_t stream) {
   if (P == 0 || I == 0) return;
   const int nv = I / 8, threads = nv >= 256 ? 256 : (nv + 31) / 32 * 32;
-  const int64_t most = (int64_t)num_sms * 32;
-  const dim3 grid((unsigned)(P < most ? P : most), P < 4 * num_sms ? (nv + threads - 1) / threads : 1);
+  const dim3 grid((unsigned)P, P < 4 * num_sms ? (nv + threads - 1) / threads : 1);
   if (half)
     swiglu_bwd_kernel<__half><<<grid, threads, 0, stream>>>(static_cast<const __half*>(da), das,
                                                             static_cast<const __half*>(z), zs,
