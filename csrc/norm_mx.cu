@@ -172,8 +172,9 @@ __global__ void __launch_bounds__(512) add_rmsnorm_mx_kernel(const NormMxArgs a)
 }
 
 // dx = r (g - s r^2 mean(g s)) + dres with g = dh w; dw = sum over rows of dh s r.
-// Each row slot of the grid (blockIdx.x, threadIdx.y) keeps its columns' sums of dw over the rows it walks;
-// part[slot] receives them, and norm_dw_kernel adds the slots in order (the result does not depend on timing).
+// Each thread row of the grid (blockIdx.x, threadIdx.y) keeps its columns' sums of dw over the rows it walks;
+// part[blockIdx.x] receives the block's, and norm_dw_kernel adds the blocks in order (the result does not depend
+// on timing).
 // Rows come through a shared-memory ring and stay packed in registers between the two passes, w stays in shared
 // memory: few registers, so that several blocks share an SM and cover each other's reductions.
 template <typename T, int THREADS, int BLOCKS>
@@ -261,15 +262,33 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rmsnorm_bwd_kernel(const Norm
       }
     }
   }
-  const int slot = blockIdx.x * group + ty;
+  // the block's rows of sums become one, in row order (the ring is drained: its memory is free)
+  float* sums = reinterpret_cast<float*>(ring.smem);
+  __syncthreads();
+  if (ty > 0) {
+#pragma unroll
+    for (int j = 0; j < kVpt; ++j) {
+      const int c = tx + j * blockDim.x;
+      if (c < nv) rows::store8f(sums + (ty - 1) * a.n + c * 8, dw[j]);
+    }
+  }
+  __syncthreads();
+  if (ty > 0) return;
 #pragma unroll
   for (int j = 0; j < kVpt; ++j) {
     const int c = tx + j * blockDim.x;
-    if (c < nv) rows::store8f(a.part + (int64_t)slot * a.n + c * 8, dw[j]);
+    if (c >= nv) continue;
+    for (int r = 1; r < group; ++r) {
+      float o[8];
+      rows::load8<float>(sums + (r - 1) * a.n + c * 8, o);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dw[j][i] += o[i];
+    }
+    rows::store8f(a.part + (int64_t)blockIdx.x * a.n + c * 8, dw[j]);
   }
 }
 
-// dw[c] = sum over slots of part[slot][c], in slot order within each of 64 fixed strands, the strands in order.
+// dw[c] = sum over slots (blocks) of part[slot][c], in slot order within each of 64 fixed strands, the strands in order.
 // Block (4 columns of float4, 64 strands): many short strands, because the sums wait on L2 latency.
 __global__ void __launch_bounds__(256) norm_dw_kernel(const float* __restrict__ part, int slots, int n,
                                                       float* __restrict__ dw) {
@@ -369,7 +388,7 @@ int rmsnorm_bwd_slots(int64_t rows, int n, bool res, int num_sms) {
   const dim3 block = norm_block(n, kVpt);
   const int64_t groups = (rows + block.y - 1) / block.y;
   const int64_t most = (int64_t)num_sms * ring_plan(n, res, block).blocks_per_sm;
-  return (int)((groups < most ? groups : most) * block.y);
+  return (int)(groups < most ? groups : most);
 }
 
 void launch_rmsnorm_bwd(const NormBwdArgs& a, int slots, cudaStream_t stream) {
@@ -380,7 +399,7 @@ void launch_rmsnorm_bwd(const NormBwdArgs& a, int slots, cudaStream_t stream) {
                    ? (a.half ? rmsnorm_bwd_kernel<__half, 256, 3> : rmsnorm_bwd_kernel<__nv_bfloat16, 256, 3>)
                    : (a.half ? rmsnorm_bwd_kernel<__half, 512, 1> : rmsnorm_bwd_kernel<__nv_bfloat16, 512, 1>);
     cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem);
-    fn<<<slots / block.y, block, p.smem, stream>>>(a, p.stages);
+    fn<<<slots, block, p.smem, stream>>>(a, p.stages);
   }
   norm_dw_kernel<<<(a.n + 15) / 16, dim3(4, 64), 0, stream>>>(a.part, slots, a.n, a.dw);
 }
