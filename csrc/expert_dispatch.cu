@@ -446,7 +446,7 @@ int launch_expert_order(const void* ids, bool wide, int64_t n, int64_t base, int
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   auto go = [&](auto* fn, auto* p) {
-    if (smem > 48 * 1024) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (smem > 40 * 1024) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (cluster > 8) cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     return (int)cudaLaunchKernelEx(&cfg, fn, p, (int)n, base, E, offsets, slots, pairs);
   };

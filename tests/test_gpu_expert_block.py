@@ -578,3 +578,13 @@ def test_block_on_the_gpu_matches_the_cpu(cuda):
         assert (a - b).norm() <= 2e-2 * b.norm()
     r = fit(tokens=512, hidden=128, inter=64, experts=8, topk=2, steps=30, lr=3e-3, device="cuda")
     assert r["last_loss"] < 0.9 * r["first_loss"]
+
+
+@pytest.mark.parametrize("E", [376, 384, 385, 500, 750, 768, 1500, 1536, 3000])
+def test_order_counters_around_the_shared_memory_default(cuda, E):
+    """Counter tables just below, at and above 48 KB (the size a launch may use without asking)."""
+    g = torch.Generator().manual_seed(E)
+    for T in (70, 1100):
+        ids = torch.randint(-1, E, (T, 8), generator=g).int()
+        for a, b in zip(dispatch.expert_order(ids.cuda(), E), dispatch.expert_order(ids, E)):
+            assert torch.equal(a.cpu(), b)
