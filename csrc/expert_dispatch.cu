@@ -403,7 +403,8 @@ void combine_typed(const CombineArgs& a, bool vec, cudaStream_t stream) {
   const int threads = nv >= 256 ? 256 : 128;
   const unsigned parts = column_parts(a.T, nv, threads, a.num_sms);
   int64_t tpb = a.T * parts / (8 * (int64_t)a.num_sms);  // tokens of a block, while every SM has eight blocks
-  tpb = tpb < 1 ? 1 : tpb > kMaxTpb ? kMaxTpb : tpb;
+  const int64_t most = a.k > 4096 / kMaxTpb ? 4096 / a.k : kMaxTpb;  // slots and weights: at most 32 KB
+  tpb = tpb < 1 ? 1 : tpb > most ? most : tpb;
   const dim3 grid((unsigned)((a.T + tpb - 1) / tpb), parts);
   const size_t smem = (size_t)tpb * a.k * 8;
   if (vec)

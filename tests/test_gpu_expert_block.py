@@ -588,3 +588,19 @@ def test_order_counters_around_the_shared_memory_default(cuda, E):
         ids = torch.randint(-1, E, (T, 8), generator=g).int()
         for a, b in zip(dispatch.expert_order(ids.cuda(), E), dispatch.expert_order(ids, E)):
             assert torch.equal(a.cpu(), b)
+
+
+@pytest.mark.parametrize("T,k", [(10000, 1000), (9000, 300), (3, 1024)])
+def test_combine_with_many_choices(cuda, T, k):
+    """A block's slots and weights stay within the shared memory of a launch at any topk."""
+    g = gen(k)
+    ids = torch.randint(-1, 40, (T, k), device="cuda", generator=g)
+    order = dispatch.expert_order(ids, 40)
+    y = randn(g, T * k, 8, dtype=BF16)
+    w = torch.rand(T, k, device="cuda", generator=g)
+    got = dispatch.combine(y, order, w, out_dtype=F32)
+    here = order.slots >= 0
+    part = torch.where(here[..., None], y[order.slots.clamp_min(0).long()].to(F64), 0.0) * torch.where(here, w, 0).to(F64)[..., None]
+    ref.check(got, part.sum(1), part.abs().sum(1) * ACC * (k + 1), "out")
+    with pytest.raises(RuntimeError, match="1024"):
+        dispatch.expert_order(torch.zeros(2, 1025, device="cuda", dtype=torch.int32), 4)
