@@ -42,9 +42,11 @@ void check_rows16(const Tensor& like, const Tensor& t, int64_t rows, int64_t n, 
   TORCH_CHECK(t.numel() == 0 || (on16(t) && row_stride(t) * t.element_size() % 16 == 0), name,
               " rows must start on 16-byte boundaries");
 }
-// t itself if its rows are contiguous and start on 16-byte boundaries, else a copy whose rows do
+// t itself if its rows are contiguous, apart from one another and on 16-byte boundaries, else a copy whose rows are
 Tensor rows16(const Tensor& t) {
-  if (t.dim() != 2 || t.numel() == 0 || (t.stride(1) == 1 && on16(t) && row_stride(t) * t.element_size() % 16 == 0)) return t;
+  if (t.dim() != 2 || t.numel() == 0 ||
+      (t.stride(1) == 1 && on16(t) && row_stride(t) >= t.size(1) && row_stride(t) * t.element_size() % 16 == 0))
+    return t;
   return t.is_contiguous() ? t.clone() : t.contiguous();
 }
 OptTensor rows16(const OptTensor& t) { return t ? OptTensor(rows16(*t)) : t; }

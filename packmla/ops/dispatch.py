@@ -140,7 +140,7 @@ class _Combine(torch.autograd.Function):
 def gather(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     """Rows [T k, H]: row r holds its pair's token row x[pairs[r] // k]; rows of no pair are zero.
 
-    x [T, H] of any type, rows contiguous (any stride between them).  Differentiable."""
+    x [T, H] of any type and strides.  Differentiable where x is BF16, FP16 or FP32."""
     _check_tokens(x, order, "x")
     if x.is_cuda:
         return ext().expert_gather(x, order.slots, order.offsets)

@@ -604,3 +604,64 @@ def test_combine_with_many_choices(cuda, T, k):
     ref.check(got, part.sum(1), part.abs().sum(1) * ACC * (k + 1), "out")
     with pytest.raises(RuntimeError, match="1024"):
         dispatch.expert_order(torch.zeros(2, 1025, device="cuda", dtype=torch.int32), 4)
+
+
+def test_broadcast_rows(cuda):
+    """One row expanded over many (stride 0): operands are read as the rows they stand for."""
+    g = gen(12)
+    row, w = randn(g, 1, 64, dtype=BF16), randn(g, 2, 32, 64, dtype=BF16)
+    offsets = spread([40, 5])
+    x = row.expand(45, 64)
+    assert torch.equal(grouped.expert_linear(x, w, offsets), grouped.expert_linear(x.contiguous(), w, offsets))
+    dy = randn(g, 1, 32, dtype=BF16).expand(45, 32)
+    for a, b in zip(grouped.expert_linear_backward(dy, x, w, offsets),
+                    grouped.expert_linear_backward(dy.contiguous(), x.contiguous(), w, offsets)):
+        assert torch.equal(a, b)
+    norm = torch.ones(64, device="cuda")
+    for a, b in zip(fused.add_rmsnorm_mx(x, norm, 1e-6, x, return_h=True),
+                    fused.add_rmsnorm_mx(x.contiguous(), norm, 1e-6, x.contiguous(), return_h=True)):
+        assert torch.equal(a, b)
+    order = routed(45, 2, 4, 0.1, 2)
+    assert torch.equal(dispatch.gather(x, order), dispatch.gather(x.contiguous(), order))
+    y = row.expand(90, 64)
+    out = dispatch.combine(y, order)
+    assert torch.equal(out, dispatch.combine(y.contiguous(), order))
+    # the gradient of a broadcast input is the sum over its rows
+    leaf = row.clone().requires_grad_(True)
+    grad, = torch.autograd.grad(dispatch.gather(leaf.expand(45, 64), order), leaf, torch.ones(90, 64, device="cuda", dtype=BF16))
+    count = float((order.slots >= 0).sum())
+    assert ((grad.float() - count).abs() <= 2 ** -7 * count).all()
+    check_errors(cuda)
+
+
+def test_offsets_past_32_bits(cuda):
+    """More than 2^31 elements and 2^32 bytes in the rows: the last rows are where they belong."""
+    T, k, H = 70000, 8, 4096
+    ids = (torch.arange(T * k, device="cuda") % 11).view(T, k)
+    order = dispatch.expert_order(ids, 11)
+    x = torch.empty(T, H, device="cuda", dtype=BF16)
+    x[:] = (torch.arange(T, device="cuda") % 251)[:, None].to(BF16)
+    x[:, -1] = 7
+    rows = dispatch.gather(x, order)
+    assert rows.numel() > 1 << 31
+    for r in (0, 1, T * k // 2, T * k - 2, T * k - 1):
+        assert torch.equal(rows[r], x[int(order.pairs[r]) // k])
+    out = dispatch.combine(rows, order)
+    for t in (0, 1, T // 2, T - 1):
+        assert torch.equal(out[t].float(), 8 * x[t].float())
+    dy, dw = dispatch.combine_backward(x, rows, order, torch.full((T, k), 2.0, device="cuda"))
+    assert torch.equal(dy[T * k - 1], 2 * x[int(order.pairs[-1]) // k])
+    last = x[T - 1].double()
+    assert abs(dw[T - 1, 0].double() - (last * last).sum()) <= 1e-5 * (last * last).sum()
+    del dy, dw, out, x
+    # products: rows x outputs past 2^31 elements
+    w = torch.zeros(2, H, 64, device="cuda", dtype=BF16)
+    w[0, :, 0], w[1, :, 1] = 1, 2
+    P = T * k
+    offsets = torch.tensor([0, P - 5, P], dtype=torch.int32, device="cuda")
+    y = grouped.expert_linear(rows[:, :64], w, offsets)
+    check_errors(cuda)
+    assert y.numel() > 1 << 31
+    for r in (0, P // 2, P - 6, P - 5, P - 1):
+        want = rows[r, 0] if r < P - 5 else 2 * rows[r, 1]
+        assert (y[r] == want).all()
