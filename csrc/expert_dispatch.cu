@@ -37,6 +37,7 @@ __global__ void __launch_bounds__(512) expert_order_kernel(const Id* __restrict_
   extern __shared__ int32_t sm[];
   __shared__ int32_t wsum[32];
   const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+  pm::griddep_launch_dependents();  // gather's blocks may be placed now; they wait for this grid's end
   cg::cluster_group cl = cg::this_cluster();
   const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
   int32_t* cnt = sm;           // [W][E]: counts, then the next row of (warp, expert)
@@ -187,6 +188,7 @@ __global__ void __launch_bounds__(256) expert_gather_kernel(const Plane rows_p, 
   const int64_t t = blockIdx.x;
   const int64_t first = (int64_t)blockIdx.y * blockDim.x + threadIdx.x, step = (int64_t)gridDim.y * blockDim.x;
   const int32_t* slot = slots + t * k;
+  pm::griddep_wait();  // (nothing is read before the grids ahead have ended)
   gather_plane<V>(rows_p, t, slot, k, n, first, step);
   if (scales_p.src) gather_plane<S>(scales_p, t, slot, k, n, first, step);
   const int64_t total = max(offsets[E], 0);
@@ -387,14 +389,20 @@ unsigned column_parts(int64_t tokens, int64_t accesses, int threads, int num_sms
 template <typename V>
 void gather_scales(const Plane& r, const Plane& s, const GatherArgs& a, cudaStream_t stream) {
   const int threads = r.bytes / (int64_t)sizeof(V) >= 256 ? 256 : 128;
-  const dim3 grid((unsigned)a.T, column_parts(a.T, r.bytes / sizeof(V), threads, a.num_sms));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)a.T, column_parts(a.T, r.bytes / sizeof(V), threads, a.num_sms));
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};  // the sort that usually precedes lets this launch overlap its end
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
   const int64_t align = s.bytes | s.src_stride | reinterpret_cast<intptr_t>(s.src);
-  if (!s.src || align % 16 == 0)
-    expert_gather_kernel<V, uint4><<<grid, threads, 0, stream>>>(r, s, a.slots, a.k, a.T * a.k, a.offsets, a.E);
-  else if (align % 4 == 0)
-    expert_gather_kernel<V, uint32_t><<<grid, threads, 0, stream>>>(r, s, a.slots, a.k, a.T * a.k, a.offsets, a.E);
-  else
-    expert_gather_kernel<V, uint8_t><<<grid, threads, 0, stream>>>(r, s, a.slots, a.k, a.T * a.k, a.offsets, a.E);
+  auto* fn = !s.src || align % 16 == 0 ? expert_gather_kernel<V, uint4>
+             : align % 4 == 0          ? expert_gather_kernel<V, uint32_t>
+                                       : expert_gather_kernel<V, uint8_t>;
+  cudaLaunchKernelEx(&cfg, fn, r, s, a.slots, a.k, a.T * a.k, a.offsets, a.E);
 }
 
 template <typename T, typename O>
