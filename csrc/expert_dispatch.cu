@@ -40,6 +40,7 @@ __global__ void __launch_bounds__(512) expert_order_kernel(const Id* __restrict_
   pm::griddep_launch_dependents();  // gather's blocks may be placed now; they wait for this grid's end
   cg::cluster_group cl = cg::this_cluster();
   const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  cl.barrier_arrive();  // waited for before this CTA writes to the others: they have all started
   int32_t* cnt = sm;           // [W][E]: counts, then the next row of (warp, expert)
   int32_t* tot = sm + W * E;   // [C][E]: every CTA's counts
   const int per = (((n + C * W - 1) / (C * W)) + 31) / 32 * 32;  // pairs of a warp
@@ -78,6 +79,7 @@ __global__ void __launch_bounds__(512) expert_order_kernel(const Id* __restrict_
     count(e, peers(e));
   }
   __syncthreads();
+  cl.barrier_wait();
   for (int e = tid; e < E; e += blockDim.x) {
     int c[16], run = 0;
 #pragma unroll
