@@ -529,6 +529,13 @@ __device__ __forceinline__ void umma2_commit_both_warp(uint64_t* bar) {
       "h"((uint16_t)3)
       : "memory");
 }
+// The same for this CTA's barrier alone.
+__device__ __forceinline__ void umma2_commit_own_warp(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+      : "memory");
+}
 // Pair loads into this CTA's shared memory (addresses from smem_u32) that complete on a barrier of either CTA of the
 // pair (`bar` from dsmem_addr); no multicast.  Warp-collective: one elected lane of a converged warp issues (from a
 // single divergent lane each load costs the issuing thread over 100 cycles, as for the MMA forms).

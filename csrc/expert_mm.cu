@@ -307,7 +307,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
       buf ^= 1;
       if (buf == 0) dph ^= 1;
     }
-    pm::umma2_commit_both_warp(drain);  // arrives once every MMA issued above has completed
+    // every MMA issued above has completed; the peer, where nobody waits for this, gets no arrival: it may be leaving
+    pm::umma2_commit_own_warp(drain);
     pm::mbar_wait_warp(pm::smem_u32(drain), 0, a.err, 407);
   } else if (MODE == kGradW && warp == kTrimWarp) {
     // ------------------------------------------------------------------ ragged rows (both CTAs)
