@@ -264,8 +264,6 @@ struct NormMxArgs {
   void* h;            // [rows, n], optional
   uint8_t* codes;     // [rows, n]
   uint8_t* scales;    // [rows, n / 32]
-  int num_sms;
-  int* err;
 };
 void launch_add_rmsnorm_mx(const NormMxArgs& a, cudaStream_t stream);
 
@@ -285,9 +283,8 @@ struct NormBwdArgs {
   float* dxf;         // [rows, n], optional: dx before its rounding
   float* part;        // workspace [slots, n]
   float* dw;          // [n]
-  int* err;
 };
-int rmsnorm_bwd_slots(int64_t rows, int n, bool res, int num_sms);
+int rmsnorm_bwd_slots(int64_t rows, int n, int num_sms);
 void launch_rmsnorm_bwd(const NormBwdArgs& a, int slots, cudaStream_t stream);
 // n codes (contiguous, a multiple of 32) with their scale bytes -> BF16.
 void launch_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t n, void* out, cudaStream_t stream);

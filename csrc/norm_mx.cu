@@ -13,9 +13,7 @@
 
 namespace {
 
-constexpr int kVpt = 2;        // 8-column vectors of a thread
 constexpr int kMaxWarps = 16;  // warps of a row (n <= 8192)
-constexpr int kMaxStages = 8;
 
 // Sum of N values over the blockDim.x threads of this thread's row (a power of two below 32, or whole warps);
 // the block's blockDim.y rows reduce side by side.  Every thread of the block calls it, and for rows of
@@ -34,72 +32,14 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*red)[kMaxWarps]) 
 #pragma unroll
     for (int i = 0; i < N; ++i) red[threadIdx.y * N + i][warp] = v[i];
   __syncthreads();
+  // every warp adds the (at most 16) partial sums by shuffles: a loop over them cost half of a row's instructions
+  const int w = threadIdx.x & 15;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    v[i] = 0.f;
-    for (int j = 0; j < warps; ++j) v[i] += red[threadIdx.y * N + i][j];
-  }
-}
-
-// A ring of row groups in shared memory: the group of blockDim.y rows that the block works on next, and those
-// after it, arrive by bulk copies while the current one is reduced and stored, so the loads in flight do
-// not depend on registers or occupancy.  Tensors follow one another in a stage, rows contiguous.
-struct RowSource {
-  const uint8_t* base;
-  int64_t stride;  // bytes between rows
-  int bytes;       // of a row (a multiple of 16)
-};
-template <int N>
-struct RowRing {
-  RowSource src[N];
-  uint8_t* smem;
-  uint64_t* full;
-  int64_t rows;
-  int stage_bytes, stages, group;
-  // stage s <- rows [row0, row0 + group) (fewer at the end; nothing past the last).  Called by warp 0.
-  __device__ __forceinline__ void issue(int s, int64_t row0, int lane) const {
-    const int64_t left = rows - row0;
-    if (left <= 0) return;
-    const int have = left < group ? (int)left : group;
-    uint32_t total = 0;
+    v[i] = w < warps ? red[threadIdx.y * N + i][w] : 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (src[i].base) total += src[i].bytes * have;
-    if (lane == 0) pm::mbar_arrive_expect_tx(full + s, total);
-    __syncwarp();
-    uint8_t* dst = smem + s * stage_bytes;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (!src[i].base) continue;
-      const uint8_t* from = src[i].base + row0 * src[i].stride;
-      if (src[i].stride == src[i].bytes) {
-        if (lane == 0) pm::bulk_g2s(dst, from, src[i].bytes * have, full + s);
-      } else {
-        for (int r = lane; r < have; r += 32) pm::bulk_g2s(dst + r * src[i].bytes, from + r * src[i].stride, src[i].bytes, full + s);
-      }
-      dst += src[i].bytes * group;
-    }
+    for (int o = 8; o >= 1; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
   }
-};
-
-// The threads of a block walk groups of blockDim.y rows: group g, g + gridDim.x, ...  `ring`: rows come through
-// the ring, else straight from global memory.
-template <int N>
-__device__ __forceinline__ void ring_start(RowRing<N>& ring, int64_t first, int64_t step) {
-  const int tid = threadIdx.y * blockDim.x + threadIdx.x;
-  if (tid == 0) {
-    for (int i = 0; i < ring.stages; ++i) pm::mbar_init(ring.full + i, 1);
-    pm::fence_mbar_init();
-  }
-  __syncthreads();
-  if (tid < 32)
-    for (int i = 0; i < ring.stages; ++i) ring.issue(i, first + i * step, tid);
-}
-
-// A wait ran out (the error word says so): let the copies in flight land before the block leaves.
-template <int N>
-__device__ __noinline__ void ring_give_up(const RowRing<N>& ring, int st, uint32_t ph) {
-  for (int s = 0; s < ring.stages; ++s) pm::mbar_wait(ring.full + s, s >= st ? ph : ph ^ 1, nullptr, 0, 20000000ull);
 }
 
 // Thread t of a row owns the 8-column vectors t, t + blockDim.x, ... (VPT of them), so the 4 lanes that share a
@@ -175,96 +115,78 @@ __global__ void __launch_bounds__(512) add_rmsnorm_mx_kernel(const NormMxArgs a)
 // Each thread row of the grid (blockIdx.x, threadIdx.y) keeps its columns' sums of dw over the rows it walks;
 // part[blockIdx.x] receives the block's, and norm_dw_kernel adds the blocks in order (the result does not depend
 // on timing).
-// Rows come through a shared-memory ring and stay packed in registers between the two passes, w stays in shared
-// memory: few registers, so that several blocks share an SM and cover each other's reductions.
-template <typename T, int THREADS, int BLOCKS>
-__global__ void __launch_bounds__(THREADS, BLOCKS) rmsnorm_bwd_kernel(const NormBwdArgs a, int stages) {
-  extern __shared__ __align__(16) uint8_t smem[];
+// A thread keeps kVpt vectors of a row packed between the two passes, and loads the next row's before it reduces the
+// current one's sums, so that the loads of every resident block are always in flight.  Bound by the instructions
+// of a row's reduction as much as by HBM: two vectors a thread take 56 us for 8192 rows of 4096 (4.8 TB/s), one
+// 70, and rows through a ring of bulk copies 66.
+constexpr int kVpt = 2;
+template <typename T>
+__global__ void __launch_bounds__(512, 1) rmsnorm_bwd_kernel(const NormBwdArgs a) {
+  extern __shared__ __align__(16) float sums[];  // [group - 1][n]
   __shared__ float red[2][2 * kMaxWarps][kMaxWarps];
-  __shared__ uint64_t full[kMaxStages];
   const int nv = a.n >> 3, tx = threadIdx.x, ty = threadIdx.y, group = blockDim.y;
-  const int tid = ty * blockDim.x + tx;
   const int64_t step = (int64_t)gridDim.x * group;
-  const int b2 = a.n * 2;
-  RowRing<3> ring;
-  ring.src[0] = {static_cast<const uint8_t*>(a.x), a.xs * 2, b2};
-  ring.src[1] = {static_cast<const uint8_t*>(a.dh), a.dhs * 2, b2};
-  ring.src[2] = {static_cast<const uint8_t*>(a.dres), a.drs * 2, b2};
-  ring.smem = smem + a.n * 4;
-  ring.full = full;
-  ring.rows = a.rows;
-  ring.stage_bytes = group * b2 * (a.dres ? 3 : 2);
-  ring.stages = stages;
-  ring.group = group;
-  ring_start(ring, (int64_t)blockIdx.x * group, step);
-  float* w = reinterpret_cast<float*>(smem);
-  for (int i = tid * 4; i < a.n; i += blockDim.x * group * 4)
-    *reinterpret_cast<float4*>(w + i) = *reinterpret_cast<const float4*>(a.w + i);
-  __syncthreads();
-  float dw[kVpt][8];
+  float w[kVpt][8], dw[kVpt][8];
+  uint4 sp[kVpt], gp[kVpt], res[kVpt];
 #pragma unroll
-  for (int j = 0; j < kVpt; ++j)
+  for (int j = 0; j < kVpt; ++j) {
+    const int c = tx + j * blockDim.x;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dw[j][i] = 0.f;
-  const float inv_n = 1.f / a.n;
-  int st = 0;
-  uint32_t ph = 0;
-  bool flip = false;
-  for (int64_t row0 = (int64_t)blockIdx.x * group; row0 < a.rows; row0 += step) {
-    const int64_t row = row0 + ty;
-    const bool live = row < a.rows;
-    const T* at = reinterpret_cast<const T*>(ring.smem + st * ring.stage_bytes) + ty * a.n;
-    if (!pm::mbar_wait(full + st, ph, tid == 0 ? a.err : nullptr, 502)) return ring_give_up(ring, st, ph);
-    uint4 sp[kVpt], gp[kVpt], res[kVpt];
-    float sum[2] = {0.f, 0.f};
+    for (int i = 0; i < 8; ++i) w[j][i] = dw[j][i] = 0.f;
+    if (c < nv) rows::load8<float>(a.w + c * 8, w[j]);
+  }
+  auto fetch = [&](int64_t row) {
 #pragma unroll
     for (int j = 0; j < kVpt; ++j) {
       const int c = tx + j * blockDim.x;
       res[j] = sp[j] = gp[j] = make_uint4(0, 0, 0, 0);
-      if (live && c < nv) {
-        sp[j] = *reinterpret_cast<const uint4*>(at + c * 8);
-        gp[j] = *reinterpret_cast<const uint4*>(at + group * a.n + c * 8);
-        if (a.dres) res[j] = *reinterpret_cast<const uint4*>(at + 2 * group * a.n + c * 8);
-        float s[8], g[8], wv[8];
-        rows::unpack8<T>(sp[j], s);
-        rows::unpack8<T>(gp[j], g);
-        rows::load8<float>(w + c * 8, wv);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          sum[0] += s[i] * s[i];
-          sum[1] += g[i] * wv[i] * s[i];
-        }
+      if (row < a.rows && c < nv) {
+        sp[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row * a.xs + c * 8);
+        gp[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.dh) + row * a.dhs + c * 8);
+        if (a.dres) res[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.dres) + row * a.drs + c * 8);
       }
     }
+  };
+  const float inv_n = 1.f / a.n;
+  bool flip = false;
+  int64_t row0 = (int64_t)blockIdx.x * group;
+  fetch(row0 + ty);
+  for (; row0 < a.rows; row0 += step) {
+    const int64_t row = row0 + ty;
+    float s[kVpt][8], g[kVpt][8], o[kVpt][8];
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < kVpt; ++j) {
+      rows::unpack8<T>(sp[j], s[j]);
+      rows::unpack8<T>(gp[j], g[j]);
+      rows::unpack8<T>(res[j], o[j]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        sum[0] = fmaf(s[j][i], s[j][i], sum[0]);
+        sum[1] = fmaf(g[j][i] * w[j][i], s[j][i], sum[1]);
+      }
+    }
+    fetch(row + step);
     row_sum<2>(sum, red[flip]);  // two buffers: a slow warp may still read the last group's sums
     flip = !flip;
-    if (blockDim.x <= 32) __syncthreads();  // (row_sum was no barrier) every thread has read this stage
-    if (tid < 32) ring.issue(st, row0 + stages * step, tid);
-    if (++st == stages) { st = 0; ph ^= 1; }
     const float r = rsqrtf(sum[0] * inv_n + a.eps);
-    const float k = sum[1] * inv_n * r * r;
+    const float k = sum[1] * inv_n * r * r * r;
 #pragma unroll
     for (int j = 0; j < kVpt; ++j) {
       const int c = tx + j * blockDim.x;
-      if (live && c < nv) {
-        float s[8], g[8], wv[8], o[8];
-        rows::unpack8<T>(sp[j], s);
-        rows::unpack8<T>(gp[j], g);
-        rows::load8<float>(w + c * 8, wv);
-        rows::unpack8<T>(res[j], o);
+      if (row < a.rows && c < nv) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          dw[j][i] += g[i] * (s[i] * r);
-          o[i] += r * (g[i] * wv[i] - s[i] * k);
+          const float t = r * g[j][i];
+          dw[j][i] = fmaf(t, s[j][i], dw[j][i]);
+          o[j][i] = fmaf(-k, s[j][i], fmaf(t, w[j][i], o[j][i]));
         }
-        *reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + row * a.n + c * 8) = rows::pack8<T>(o);
-        if (a.dxf) rows::store8f(a.dxf + row * a.n + c * 8, o);
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + row * a.n + c * 8) = rows::pack8<T>(o[j]);
+        if (a.dxf) rows::store8f(a.dxf + row * a.n + c * 8, o[j]);
       }
     }
   }
-  // the block's rows of sums become one, in row order (the ring is drained: its memory is free)
-  float* sums = reinterpret_cast<float*>(ring.smem);
-  __syncthreads();
+  // the block's rows of sums become one, in row order
   if (ty > 0) {
 #pragma unroll
     for (int j = 0; j < kVpt; ++j) {
@@ -278,11 +200,11 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) rmsnorm_bwd_kernel(const Norm
   for (int j = 0; j < kVpt; ++j) {
     const int c = tx + j * blockDim.x;
     if (c >= nv) continue;
-    for (int r = 1; r < group; ++r) {
-      float o[8];
-      rows::load8<float>(sums + (r - 1) * a.n + c * 8, o);
+    for (int q = 1; q < group; ++q) {
+      float t[8];
+      rows::load8<float>(sums + (q - 1) * a.n + c * 8, t);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) dw[j][i] += o[i];
+      for (int i = 0; i < 8; ++i) dw[j][i] += t[i];
     }
     rows::store8f(a.part + (int64_t)blockIdx.x * a.n + c * 8, dw[j]);
   }
@@ -344,26 +266,8 @@ dim3 norm_block(int n, int vpt) {
   const int ty = tx >= 256 ? 1 : 256 / tx;
   return dim3(tx, ty);
 }
-// Ring of a gradient block: blocks of an SM by warps and registers (the kernel's launch bounds: 80 a thread with at
-// most 256 threads, so 6 warps on each quarter of an SM, else 128), then as many stages as their shared
-// memory holds, two at least.
-struct RingPlan {
-  int stages, smem, blocks_per_sm;
-};
-RingPlan ring_plan(int n, bool res, const dim3& block) {
-  const int stage = (int)block.y * n * 2 * (res ? 3 : 2), w = n * 4, whole = 208 * 1024;
-  RingPlan p;
-  const int threads = block.x * block.y;
-  p.blocks_per_sm = (threads <= 256 ? 24 : 16) * 32 / threads;
-  while (p.blocks_per_sm > 1 && whole / p.blocks_per_sm - 5 * 1024 - w < 2 * stage) --p.blocks_per_sm;
-  p.stages = (whole / p.blocks_per_sm - 5 * 1024 - w) / stage;
-  p.stages = p.stages > kMaxStages ? kMaxStages : p.stages;
-  p.smem = w + p.stages * stage;
-  return p;
-}
-
-// Vectors of a thread by width: one up to 4096 columns (74 us for 8192 rows of 4096 against 77 with two, 2.8 us
-// against 3.6 for 8 rows: half the serial work of a thread), two beyond (512 threads).
+// Vectors of a thread by width: one up to 4096 columns (73 us, 6.0 TB/s, for 8192 rows of 4096 against 77 with two,
+// 2.7 us against 3.6 for 8 rows: half the serial work of a thread), two beyond (512 threads).
 template <int VPT>
 void launch_fwd(const NormMxArgs& a, cudaStream_t stream) {
   const dim3 block = norm_block(a.n, VPT);
@@ -384,22 +288,18 @@ void launch_add_rmsnorm_mx(const NormMxArgs& a, cudaStream_t stream) {
     launch_fwd<2>(a, stream);
 }
 
-int rmsnorm_bwd_slots(int64_t rows, int n, bool res, int num_sms) {
+int rmsnorm_bwd_slots(int64_t rows, int n, int num_sms) {
   const dim3 block = norm_block(n, kVpt);
-  const int64_t groups = (rows + block.y - 1) / block.y;
-  const int64_t most = (int64_t)num_sms * ring_plan(n, res, block).blocks_per_sm;
+  // resident blocks: 512 threads an SM (the kernel's 128 registers)
+  const int64_t groups = (rows + block.y - 1) / block.y, most = (int64_t)num_sms * (512 / (int)(block.x * block.y));
   return (int)(groups < most ? groups : most);
 }
 
 void launch_rmsnorm_bwd(const NormBwdArgs& a, int slots, cudaStream_t stream) {
   const dim3 block = norm_block(a.n, kVpt);
   if (slots > 0) {
-    const RingPlan p = ring_plan(a.n, a.dres != nullptr, block);
-    auto* fn = block.x * block.y <= 256
-                   ? (a.half ? rmsnorm_bwd_kernel<__half, 256, 3> : rmsnorm_bwd_kernel<__nv_bfloat16, 256, 3>)
-                   : (a.half ? rmsnorm_bwd_kernel<__half, 512, 1> : rmsnorm_bwd_kernel<__nv_bfloat16, 512, 1>);
-    cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem);
-    fn<<<slots, block, p.smem, stream>>>(a, p.stages);
+    auto* fn = a.half ? rmsnorm_bwd_kernel<__half> : rmsnorm_bwd_kernel<__nv_bfloat16>;
+    fn<<<slots, block, (block.y - 1) * a.n * sizeof(float), stream>>>(a);
   }
   norm_dw_kernel<<<(a.n + 15) / 16, dim3(4, 64), 0, stream>>>(a.part, slots, a.n, a.dw);
 }

@@ -73,9 +73,8 @@ void check_norm(const Tensor& x, const char* op) {
 // -> (stream, codes, scales, h or None); stream is x itself without addends or in place
 std::tuple<Tensor, Tensor, Tensor, OptTensor> add_rmsnorm_mx(const Tensor& x_in, const Tensor& w, double eps,
                                                              const OptTensor& d_in, const OptTensor& df_in, bool inplace,
-                                                             bool return_h, const Tensor& err) {
+                                                             bool return_h) {
   check_norm(x_in, "add_rmsnorm_mx");
-  check_err(x_in, err);
   const Tensor x = inplace ? x_in : rows16(x_in);
   const OptTensor d = rows16(d_in), df = rows16(df_in);
   const int64_t rows = x.size(0), n = x.size(1);
@@ -104,8 +103,6 @@ std::tuple<Tensor, Tensor, Tensor, OptTensor> add_rmsnorm_mx(const Tensor& x_in,
   if (h) a.h = h->data_ptr();
   a.codes = codes.data_ptr<uint8_t>();
   a.scales = scales.data_ptr<uint8_t>();
-  a.num_sms = sms(x);
-  a.err = err.data_ptr<int>();
   launch_add_rmsnorm_mx(a, stream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {s, codes, scales, h};
@@ -113,10 +110,8 @@ std::tuple<Tensor, Tensor, Tensor, OptTensor> add_rmsnorm_mx(const Tensor& x_in,
 
 // -> (dx in x's type, dw fp32, dx in fp32 or None)
 std::tuple<Tensor, Tensor, OptTensor> rmsnorm_backward(const Tensor& dh_in, const Tensor& x_in, const Tensor& w,
-                                                       double eps, const OptTensor& dres_in, bool fp32_dx,
-                                                       const Tensor& err) {
+                                                       double eps, const OptTensor& dres_in, bool fp32_dx) {
   check_norm(x_in, "add_rmsnorm_backward");
-  check_err(x_in, err);
   const Tensor x = rows16(x_in), dh = rows16(dh_in);
   const OptTensor dres = rows16(dres_in);
   const int64_t rows = x.size(0), n = x.size(1);
@@ -125,7 +120,7 @@ std::tuple<Tensor, Tensor, OptTensor> rmsnorm_backward(const Tensor& dh_in, cons
   check_weight(x, w, n);
   if (dres) check_rows16(x, *dres, rows, n, x.scalar_type(), "dres");
   const c10::cuda::CUDAGuard g(x.device());
-  const int slots = rmsnorm_bwd_slots(rows, (int)n, dres.has_value(), sms(x));
+  const int slots = rmsnorm_bwd_slots(rows, (int)n, sms(x));
   Tensor dx = make({rows, n}, x), dw = make({n}, x, torch::kFloat32);
   Tensor part = make({slots, n}, x, torch::kFloat32);
   OptTensor dxf;
@@ -145,7 +140,6 @@ std::tuple<Tensor, Tensor, OptTensor> rmsnorm_backward(const Tensor& dh_in, cons
   if (dxf) a.dxf = dxf->data_ptr<float>();
   a.part = part.data_ptr<float>();
   a.dw = dw.data_ptr<float>();
-  a.err = err.data_ptr<int>();
   launch_rmsnorm_bwd(a, slots, stream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {dx, dw, dxf};
@@ -430,9 +424,9 @@ OptTensor some(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(
 
 struct AddRmsNormMx : Function<AddRmsNormMx> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& d,
-                               const OptTensor& df, double eps, bool return_h, const Tensor& err) {
-    auto [s, codes, scales, h] = add_rmsnorm_mx(x, w, eps, d, df, false, return_h, err);
-    ctx->save_for_backward({s, w, err});
+                               const OptTensor& df, double eps, bool return_h) {
+    auto [s, codes, scales, h] = add_rmsnorm_mx(x, w, eps, d, df, false, return_h);
+    ctx->save_for_backward({s, w});
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["d"] = d.has_value();
     ctx->saved_data["df"] = df.has_value();
@@ -449,14 +443,14 @@ struct AddRmsNormMx : Function<AddRmsNormMx> {
     const Tensor ds = g[0], dh = g.size() > 3 ? g[3] : Tensor();
     Tensor dx = ds, dw, dxf;
     if (dh.defined()) {
-      auto [a, b, c] = rmsnorm_backward(dh, saved[0], saved[1], ctx->saved_data["eps"].toDouble(), some(ds), has_f, saved[2]);
+      auto [a, b, c] = rmsnorm_backward(dh, saved[0], saved[1], ctx->saved_data["eps"].toDouble(), some(ds), has_f);
       dx = a;
       dw = b;
       if (c) dxf = *c;
     } else if (has_f && ds.defined()) {
       dxf = ds.to(torch::kFloat32);  // only the stream was used
     }
-    return {dx, dw, has_d ? dx : Tensor(), dxf, Tensor(), Tensor(), Tensor()};
+    return {dx, dw, has_d ? dx : Tensor(), dxf, Tensor(), Tensor()};
   }
 };
 
@@ -517,10 +511,10 @@ struct ExpertLinear : Function<ExpertLinear> {
 
 std::tuple<Tensor, Tensor, Tensor, OptTensor> add_rmsnorm_mx_op(const Tensor& x, const Tensor& w, double eps,
                                                                 const OptTensor& d, const OptTensor& df, bool inplace,
-                                                                bool return_h, const Tensor& err) {
-  if (!wanted({&x, &w, at_or_null(d), at_or_null(df)})) return add_rmsnorm_mx(x, w, eps, d, df, inplace, return_h, err);
+                                                                bool return_h) {
+  if (!wanted({&x, &w, at_or_null(d), at_or_null(df)})) return add_rmsnorm_mx(x, w, eps, d, df, inplace, return_h);
   TORCH_CHECK(!inplace, "add_rmsnorm_mx: inplace is not available where a gradient is recorded");
-  variable_list o = AddRmsNormMx::apply(x, w, d, df, eps, return_h, err);
+  variable_list o = AddRmsNormMx::apply(x, w, d, df, eps, return_h);
   return {o[0], o[1], o[2], return_h ? OptTensor(o[3]) : OptTensor()};
 }
 Tensor gather_op(const Tensor& x, const Tensor& slots, const Tensor& offsets) {

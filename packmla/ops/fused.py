@@ -6,7 +6,7 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from ..formats import abi, codec
-from ._ext import error_word, ext
+from ._ext import ext
 
 
 def add_rmsnorm(x: torch.Tensor, w: torch.Tensor, eps: float, d: torch.Tensor | None = None,
@@ -148,7 +148,7 @@ def add_rmsnorm_backward(dh: torch.Tensor, x: torch.Tensor, w: torch.Tensor, eps
     Returns (dx, dw) - dx in x's type is also the gradient of the addend d, dw is fp32 and does not depend on
     timing (fixed summation order) - or (dx, dw, fp32 dx) with `fp32_dx`, the gradient of the fp32 addend."""
     if x.is_cuda:
-        dx, dw, dxf = ext().rmsnorm_backward(dh, x, w, eps, dres, fp32_dx, error_word(x.device))
+        dx, dw, dxf = ext().rmsnorm_backward(dh, x, w, eps, dres, fp32_dx)
         return (dx, dw, dxf) if fp32_dx else (dx, dw)
     _check_norm(x, w)
     n, r = _norm_oracle(x.float(), w, eps)
@@ -200,11 +200,11 @@ def add_rmsnorm_mx(x: torch.Tensor, w: torch.Tensor, eps: float, d: torch.Tensor
     Differentiable in x, w, d and dfp32 through x_new and h; the codes carry no gradient (a trainer that feeds
     them to its products uses h's gradient for them)."""
     if x.is_cuda and not inplace:
-        return ext().add_rmsnorm_mx(x, w, eps, d, dfp32, False, return_h, error_word(x.device))
+        return ext().add_rmsnorm_mx(x, w, eps, d, dfp32, False, return_h)
     wanted = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, d, dfp32))
     if not wanted:
         if x.is_cuda:
-            return ext().add_rmsnorm_mx(x, w, eps, d, dfp32, True, return_h, error_word(x.device))
+            return ext().add_rmsnorm_mx(x, w, eps, d, dfp32, True, return_h)
         return _add_rmsnorm_mx(x, w, eps, d, dfp32, inplace, return_h)
     if inplace:
         raise ValueError("inplace is not available where a gradient is recorded")
