@@ -19,6 +19,16 @@ Tensor make(at::IntArrayRef size, const Tensor& like, torch::ScalarType type) {
   return at::detail::empty_cuda(size, type, like.device(), c10::nullopt);
 }
 Tensor make(at::IntArrayRef size, const Tensor& like) { return make(size, like, like.scalar_type()); }
+// A contiguous tensor of its own inside `whole`'s memory, `at` bytes in: tensors that live and die together (the
+// tables of an order; codes and their scales) come from one allocation, which is most of a small call's cost.
+Tensor part_of(const Tensor& whole, int64_t at, at::IntArrayRef size, torch::ScalarType type) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(),
+                                                      c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_storage_offset(at / (int64_t)c10::elementSize(type));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(size);
+  return t;
+}
+int64_t up16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 bool is16(const Tensor& t) { return t.scalar_type() == torch::kBFloat16 || t.scalar_type() == torch::kFloat16; }
 bool on16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 // a row of a two-dimensional tensor that has one row may report any stride
@@ -85,8 +95,9 @@ std::tuple<Tensor, Tensor, Tensor, OptTensor> add_rmsnorm_mx(const Tensor& x_in,
   const c10::cuda::CUDAGuard g(x.device());
   const bool add = d || df;
   Tensor s = add && !inplace ? make({rows, n}, x) : x_in;
-  Tensor codes = make({rows, n}, x, torch::kUInt8);
-  Tensor scales = make({rows, n / 32}, x, torch::kUInt8);
+  const Tensor mx = make({rows * n + rows * (n / 32)}, x, torch::kUInt8);
+  Tensor codes = part_of(mx, 0, {rows, n}, torch::kUInt8);
+  Tensor scales = part_of(mx, rows * n, {rows, n / 32}, torch::kUInt8);
   OptTensor h;
   if (return_h) h = make({rows, n}, x);
   NormMxArgs a{};
@@ -170,8 +181,10 @@ std::tuple<Tensor, Tensor, Tensor> expert_order(const Tensor& ids_in, int64_t nu
   const int64_t T = ids.size(0), k = ids.size(1);
   const auto i32 = ids.options().dtype(torch::kInt32);
   if (T * k == 0) return {torch::zeros({num_experts + 1}, i32), torch::empty({T, k}, i32), torch::empty({0}, i32)};
-  Tensor offsets = make({num_experts + 1}, ids, torch::kInt32), slots = make({T, k}, ids, torch::kInt32),
-         pairs = make({T * k}, ids, torch::kInt32);
+  const int64_t table = up16(T * k * 4);
+  const Tensor whole = make({2 * table + (num_experts + 1) * 4}, ids, torch::kUInt8);
+  Tensor slots = part_of(whole, 0, {T, k}, torch::kInt32), pairs = part_of(whole, table, {T * k}, torch::kInt32);
+  Tensor offsets = part_of(whole, 2 * table, {num_experts + 1}, torch::kInt32);
   const int rc = launch_expert_order(ids.data_ptr(), ids.scalar_type() == torch::kInt64, T * k, expert_base,
                                      (int)num_experts, offsets.data_ptr<int32_t>(),
                                      slots.data_ptr<int32_t>(), pairs.data_ptr<int32_t>(), stream());
