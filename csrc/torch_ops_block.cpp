@@ -508,7 +508,8 @@ struct ExpertLinear : Function<ExpertLinear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& offsets, bool gated,
                         const Tensor& err) {
     auto [y, pre] = expert_mm(x, w, offsets, gated, gated, err);
-    ctx->save_for_backward({x, w, offsets, pre ? *pre : Tensor(), err});
+    ctx->save_for_backward({x, w, offsets, pre ? *pre : Tensor()});
+    ctx->saved_data["err"] = err;  // not a saved variable: the host clears it in place between the passes
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
@@ -516,7 +517,7 @@ struct ExpertLinear : Function<ExpertLinear> {
     const auto saved = ctx->get_saved_variables();
     const Tensor dz = saved[3].defined() ? swiglu_backward(g[0], saved[3], saved[2]) : g[0];
     auto [dx, dw] = expert_mm_backward(dz, saved[0], saved[1], saved[2], ctx->needs_input_grad(0),
-                                       ctx->needs_input_grad(1), saved[4]);
+                                       ctx->needs_input_grad(1), ctx->saved_data["err"].toTensor());
     return {dx ? *dx : Tensor(), dw ? *dw : Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };

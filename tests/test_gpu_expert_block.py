@@ -665,3 +665,16 @@ def test_offsets_past_32_bits(cuda):
     for r in (0, P // 2, P - 6, P - 5, P - 1):
         want = rows[r, 0] if r < P - 5 else 2 * rows[r, 1]
         assert (y[r] == want).all()
+
+
+@pytest.mark.parametrize("activation", [None, "swiglu"])
+def test_error_check_between_the_passes(cuda, activation):
+    """`check_errors` clears the error word in place; a backward pass after it still runs."""
+    g = gen(21)
+    x, w = randn(g, 40, 64, dtype=BF16).requires_grad_(True), randn(g, 2, 32, 64, dtype=BF16).requires_grad_(True)
+    out = grouped.expert_linear(x, w, spread([30, 10]), activation)
+    v = randn(g, *out.shape, dtype=BF16)
+    want = torch.autograd.grad(out, (x, w), v, retain_graph=True)
+    check_errors(cuda)
+    for a, b in zip(torch.autograd.grad(out, (x, w), v), want):
+        assert torch.equal(a, b)
