@@ -22,7 +22,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 // ----------------------------------------------------------------------------- order
-// A stable counting sort in one launch: the CTAs of one cluster (1 to 8) take consecutive ranges of pairs, the
+// A stable counting sort in one launch: the CTAs of one cluster (1 to 16) take consecutive ranges of pairs, the
 // warps of a CTA consecutive ranges of its range.  Pass 1 counts per warp (one lane of those with equal experts
 // adds: no atomics), the counts become starting rows (over warps, then CTAs, then experts), pass 2 hands out
 // rows in the same order.  Latency bound: a lane's first kHeld ids and its peers of equal expert stay in
@@ -441,9 +441,9 @@ int launch_expert_order(const void* ids, bool wide, int64_t n, int64_t base, int
   while (cluster < 16 && (int64_t)cluster * 512 < n) cluster *= 2;
   int warps = (int)((n + 32 * cluster - 1) / (32 * cluster));
   warps = warps < 4 ? 4 : warps > 16 ? 16 : warps;
-  const int most = 200 * 1024 / 4 / E - cluster;  // shared memory: (warps + CTAs) counters of every expert
-  while (cluster > 1 && 200 * 1024 / 4 / E - cluster < 8) cluster /= 2;
-  warps = warps > most ? most : warps;
+  const int counters = 200 * 1024 / 4 / E;  // shared memory: (warps + CTAs) counters of every expert
+  while (cluster > 1 && counters - cluster < 8) cluster /= 2;
+  warps = warps > counters - cluster ? counters - cluster : warps;
   if (warps < 1) return -1;
   const size_t smem = (size_t)(warps + cluster) * E * sizeof(int32_t);
   cudaLaunchConfig_t cfg{};

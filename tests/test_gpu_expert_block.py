@@ -678,3 +678,13 @@ def test_error_check_between_the_passes(cuda, activation):
     check_errors(cuda)
     for a, b in zip(torch.autograd.grad(out, (x, w), v), want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("E", [2049, 3011, 3012, 3600, 4096])
+def test_order_of_many_pairs_and_experts(cuda, E):
+    """Where the counters of all sixteen blocks and warps would not fit, fewer of them sort the pairs."""
+    g = torch.Generator().manual_seed(E)
+    for T in (300, 600, 1100, 9000):
+        ids = torch.randint(-1, E, (T, 8), generator=g).int()
+        for a, b in zip(dispatch.expert_order(ids.cuda(), E), dispatch.expert_order(ids, E)):
+            assert torch.equal(a.cpu(), b)
