@@ -38,6 +38,9 @@ int64_t row_stride(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stri
 // and torch were linked with different C++ runtimes.
 std::string num(int64_t v) { return std::to_string(v); }
 
+// Rows of adjacent elements: a column of one element may report any stride.
+bool dense_rows(const Tensor& t) { return t.numel() == 0 || t.size(1) == 1 || t.stride(1) == 1; }
+
 void check_device(const Tensor& like, const Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", like.device());
 }
@@ -45,7 +48,7 @@ void check_rows(const Tensor& like, const Tensor& t, int64_t rows, int64_t n, to
   check_device(like, t, name);
   TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == n, name, " must be [", num(rows), ", ", num(n), "]");
   TORCH_CHECK(t.scalar_type() == type, name, " must be ", type);
-  TORCH_CHECK(t.numel() == 0 || t.stride(1) == 1, name, " rows must be contiguous");
+  TORCH_CHECK(dense_rows(t), name, " rows must be contiguous");
 }
 void check_rows16(const Tensor& like, const Tensor& t, int64_t rows, int64_t n, torch::ScalarType type, const char* name) {
   check_rows(like, t, rows, n, type, name);
@@ -61,7 +64,7 @@ Tensor rows16(const Tensor& t) {
 }
 OptTensor rows16(const OptTensor& t) { return t ? OptTensor(rows16(*t)) : t; }
 // t itself if its rows are contiguous, else a copy
-Tensor packed_rows(const Tensor& t) { return t.dim() != 2 || t.numel() == 0 || t.stride(1) == 1 ? t : t.contiguous(); }
+Tensor packed_rows(const Tensor& t) { return t.dim() != 2 || dense_rows(t) ? t : t.contiguous(); }
 OptTensor packed_rows(const OptTensor& t) { return t ? OptTensor(packed_rows(*t)) : t; }
 void check_err(const Tensor& like, const Tensor& err) {
   check_device(like, err, "err");

@@ -688,3 +688,17 @@ def test_order_of_many_pairs_and_experts(cuda, E):
         ids = torch.randint(-1, E, (T, 8), generator=g).int()
         for a, b in zip(dispatch.expert_order(ids.cuda(), E), dispatch.expert_order(ids, E)):
             assert torch.equal(a.cpu(), b)
+
+
+def test_one_column_of_any_stride(cuda):
+    """A [rows, 1] view (top-1 weights, one-wide rows) is dense whatever stride its column reports."""
+    order = routed(37, 1, 4, 0.2, 5)
+    g = gen(31)
+    y, dout = randn(g, 37, 24, dtype=BF16), randn(g, 37, 24, dtype=BF16)
+    w = randn(g, 3, 37)[:1].t()
+    assert w.stride(1) != 1
+    assert torch.equal(dispatch.combine(y, order, w), dispatch.combine(y, order, w.clone(memory_format=torch.contiguous_format)))
+    for a, b in zip(dispatch.combine_backward(dout, y, order, w), dispatch.combine_backward(dout, y, order, w.reshape(37).clone()[:, None])):
+        assert torch.equal(a, b)
+    x = randn(g, 3, 37)[:1].t()
+    assert torch.equal(dispatch.gather(x, order), dispatch.gather(x.reshape(37).clone()[:, None], order))
