@@ -1,6 +1,7 @@
 // Torch-facing wrappers of the mixture-of-experts block operators (norm_mx.cu, expert_dispatch.cu,
 // expert_mm.cu): argument validation, output allocation, then the plain launchers.
 #include <torch/extension.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -95,8 +96,14 @@ std::tuple<Tensor, Tensor, Tensor, OptTensor> add_rmsnorm_mx(const Tensor& x_in,
   check_weight(x, w, n);
   if (d) check_rows16(x, *d, rows, n, x.scalar_type(), "d");
   if (df) check_rows16(x, *df, rows, n, torch::kFloat32, "dfp32");
-  const c10::cuda::CUDAGuard g(x.device());
   const bool add = d || df;
+  if (inplace && add) {
+    TORCH_CHECK(rows <= 1 || row_stride(x) >= n, "add_rmsnorm_mx: inplace needs rows apart from one another");
+    TORCH_CHECK(!d_in || at::get_overlap_status(x, *d_in) != at::MemOverlapStatus::Partial,
+                "add_rmsnorm_mx: d and the x that is written over overlap in part");
+    x.unsafeGetTensorImpl()->bump_version();  // a gradient that saved x's old values must not use the new ones
+  }
+  const c10::cuda::CUDAGuard g(x.device());
   Tensor s = add && !inplace ? make({rows, n}, x) : x_in;
   const Tensor mx = make({rows * n + rows * (n / 32)}, x, torch::kUInt8);
   Tensor codes = part_of(mx, 0, {rows, n}, torch::kUInt8);

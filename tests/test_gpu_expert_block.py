@@ -702,3 +702,28 @@ def test_one_column_of_any_stride(cuda):
         assert torch.equal(a, b)
     x = randn(g, 3, 37)[:1].t()
     assert torch.equal(dispatch.gather(x, order), dispatch.gather(x.reshape(37).clone()[:, None], order))
+
+
+def test_norm_inplace_is_seen_and_checked(cuda):
+    """An in-place sum counts as a change of x: a gradient that saved x's old values refuses; overlapping rows are refused."""
+    g = gen(41)
+    w, d = torch.ones(64, device="cuda"), randn(g, 8, 64, dtype=BF16)
+    x = randn(g, 8, 64, dtype=BF16)
+    scale = torch.ones(64, device="cuda", dtype=BF16, requires_grad=True)
+    y = x * scale  # saves x
+    new, *_ = fused.add_rmsnorm_mx(x, w, 1e-6, d, inplace=True)
+    assert new.data_ptr() == x.data_ptr()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with pytest.raises(RuntimeError, match="apart"):
+        fused.add_rmsnorm_mx(x[:1].expand(8, 64), w, 1e-6, d, inplace=True)
+    with pytest.raises(RuntimeError, match="apart"):
+        fused.add_rmsnorm_mx(torch.as_strided(x, (8, 64), (32, 1)), w, 1e-6, d, inplace=True)
+    flat = randn(g, 9 * 64, dtype=BF16)
+    with pytest.raises(RuntimeError, match="overlap"):
+        fused.add_rmsnorm_mx(flat[:512].view(8, 64), w, 1e-6, flat[64:].view(8, 64), inplace=True)
+    with torch.inference_mode():
+        a = randn(g, 8, 64, dtype=BF16)
+        b = a.clone()
+        new, *_ = fused.add_rmsnorm_mx(a, w, 1e-6, d, inplace=True)
+        assert torch.equal(new, fused.add_rmsnorm_mx(b, w, 1e-6, d)[0])
