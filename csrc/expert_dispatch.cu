@@ -260,63 +260,59 @@ struct Raw {
   }
 };
 
-// Block (tokens [tpb b, tpb (b + 1)), column part): thread c of the part sums its NV columns over each token's
-// choices.  The tokens' slots and weights are fetched together first, so that no row load waits for its slot.
-constexpr int kMaxTpb = 16;    // tokens of a block
-
+// Block (token, column part): thread c of the part sums its NV columns over the token's choices.  The token's slots
+// and weights are fetched together first, so that no row load waits for its slot.
 template <typename T, typename O, int NV>
-__global__ void __launch_bounds__(256) expert_combine_kernel(const CombineArgs a, int tpb) {
-  extern __shared__ int32_t sm[];
-  float* wt = reinterpret_cast<float*>(sm + tpb * a.k);
-  const int64_t t0 = (int64_t)blockIdx.x * tpb;
-  const int tokens = (int)min((int64_t)tpb, a.T - t0), nv = a.width / NV, k = a.k;
-  for (int i = threadIdx.x; i < tokens * k; i += blockDim.x) {
-    const int r = a.slots[t0 * k + i];
-    sm[i] = has_row(r, a.T * k) ? r : -1;
-    wt[i] = a.weights ? a.weights[(t0 + i / k) * a.ws + i % k] : 1.f;
+__global__ void __launch_bounds__(128) expert_combine_kernel(const CombineArgs a) {
+  extern __shared__ int32_t slots[];
+  float* wt = reinterpret_cast<float*>(slots + a.k);
+  const int64_t t = blockIdx.x;
+  const int nv = a.width / NV, k = a.k;
+  for (int i = threadIdx.x; i < k; i += blockDim.x) {
+    const int r = a.slots[t * k + i];
+    slots[i] = has_row(r, a.T * k) ? r : -1;
+    wt[i] = a.weights ? a.weights[t * a.ws + i] : 1.f;
   }
   __syncthreads();
   const T* y = static_cast<const T*>(a.y);
   const int step = gridDim.y * blockDim.x;
-  for (int t = 0; t < tokens; ++t) {
-    for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < nv; c += step) {
-      const int64_t col = (int64_t)c * NV;
-      float acc[NV];
-      if (a.residual) {
-        Raw<O, NV> res;
-        res.load(static_cast<const O*>(a.residual) + (t0 + t) * a.rs + col);
-        res.get(acc);
-      } else {
+  for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < nv; c += step) {
+    const int64_t col = (int64_t)c * NV;
+    float acc[NV];
+    if (a.residual) {
+      Raw<O, NV> res;
+      res.load(static_cast<const O*>(a.residual) + t * a.rs + col);
+      res.get(acc);
+    } else {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) acc[i] = 0.f;
-      }
-      for (int j0 = 0; j0 < k; j0 += kBatch) {
-        const int32_t* slot = sm + t * k + j0;
-        const float* w = wt + t * k + j0;
-        Raw<T, NV> v[kBatch];
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j)
-          if (j0 + j < k && slot[j] >= 0) v[j].load(y + (int64_t)slot[j] * a.ys + col);
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j)
-          if (j0 + j < k && slot[j] >= 0) {  // a pair without a row adds nothing, whatever its weight holds
-            float f[NV];
-            v[j].get(f);
-#pragma unroll
-            for (int i = 0; i < NV; ++i) acc[i] = fmaf(w[j], f[i], acc[i]);
-          }
-      }
-      store_n<O, NV>(static_cast<O*>(a.out) + (t0 + t) * a.width + col, acc);
+      for (int i = 0; i < NV; ++i) acc[i] = 0.f;
     }
+    for (int j0 = 0; j0 < k; j0 += kBatch) {
+      const int32_t* slot = slots + j0;
+      const float* w = wt + j0;
+      Raw<T, NV> v[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (j0 + j < k && slot[j] >= 0) v[j].load(y + (int64_t)slot[j] * a.ys + col);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (j0 + j < k && slot[j] >= 0) {  // a pair without a row adds nothing, whatever its weight holds
+          float f[NV];
+          v[j].get(f);
+#pragma unroll
+          for (int i = 0; i < NV; ++i) acc[i] = fmaf(w[j], f[i], acc[i]);
+        }
+    }
+    store_n<O, NV>(static_cast<O*>(a.out) + t * a.width + col, acc);
   }
 }
 
 // Block per token, the last token first: the rows that the forward pass read last may still be in L2.  dout's
 // columns are read once, every choice's y row once; the k dot products end in one block reduction per batch of
-// choices.
+// choices.  Loads of a batch of rows before the stores of another: 94.6 us for 4096 x 8 rows of 4096, 107 by turns.
 template <typename T, typename O, int NV>
-__global__ void __launch_bounds__(256) expert_combine_bwd_kernel(const CombineBwdArgs a) {
-  __shared__ float red[kBatch][8];
+__global__ void __launch_bounds__(128) expert_combine_bwd_kernel(const CombineBwdArgs a) {
+  __shared__ float red[kBatch][4];
   const int64_t t = (int64_t)gridDim.x - 1 - blockIdx.x;
   const int nv = a.width / NV, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int32_t* slot = a.slots + t * a.k;
@@ -336,31 +332,41 @@ __global__ void __launch_bounds__(256) expert_combine_bwd_kernel(const CombineBw
       dot[j] = 0.f;
     }
     for (int c = threadIdx.x; c < nv; c += blockDim.x) {
-      float d[NV];
+      float d[NV], v[NV];
+      Raw<T, NV> in[kBatch];  // all loaded before the first store, which no load may pass
       load_n<O, NV>(g + (int64_t)c * NV, d);
+      if (a.dw) {
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        if (r[j] < 0) continue;
-        float v[NV];
-        if (a.dw) {
-          load_n<T, NV>(y + (int64_t)r[j] * a.ys + (int64_t)c * NV, v);
+        for (int j = 0; j < kBatch; ++j)
+          if (r[j] >= 0) in[j].load(y + (int64_t)r[j] * a.ys + (int64_t)c * NV);
+      }
+      if (dy) {
 #pragma unroll
-          for (int i = 0; i < NV; ++i) dot[j] = fmaf(d[i], v[i], dot[j]);
-        }
-        if (dy) {
+        for (int j = 0; j < kBatch; ++j)
+          if (r[j] >= 0) {
 #pragma unroll
-          for (int i = 0; i < NV; ++i) v[i] = w[j] * d[i];
-          store_n<T, NV>(dy + (int64_t)r[j] * a.width + (int64_t)c * NV, v);
-        }
+            for (int i = 0; i < NV; ++i) v[i] = w[j] * d[i];
+            store_n<T, NV>(dy + (int64_t)r[j] * a.width + (int64_t)c * NV, v);
+          }
+      }
+      if (a.dw) {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+          if (r[j] >= 0) {
+            in[j].get(v);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) dot[j] = fmaf(d[i], v[i], dot[j]);
+          }
       }
     }
     if (a.dw) {
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
+      for (int j = 0; j < kBatch; ++j)
+        if (j0 + j < a.k) {
 #pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
-        if (lane == 0) red[j][warp] = dot[j];
-      }
+          for (int o = 16; o >= 1; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
+          if (lane == 0) red[j][warp] = dot[j];
+        }
       __syncthreads();
       if (threadIdx.x < kBatch && j0 + threadIdx.x < a.k) {
         float s = 0.f;
@@ -409,26 +415,25 @@ void gather_scales(const Plane& r, const Plane& s, const GatherArgs& a, cudaStre
 
 template <typename T, typename O>
 void combine_typed(const CombineArgs& a, bool vec, cudaStream_t stream) {
+  // 128 threads: 6001 x 6 rows of 2048 take 32.0 us (5.4 TB/s) against 35.4 with 256, 1024 x 8 of 4096 15.7 against
+  // 16.7, 8192 x 8 of 4096 92.8 (6.5 TB/s) either way; blocks of several tokens gain nothing
   const int nv = vec ? a.width / 8 : a.width;
-  const int threads = nv >= 256 ? 256 : 128;
-  const unsigned parts = column_parts(a.T, nv, threads, a.num_sms);
-  // tokens of a block, while every SM has sixteen blocks (8192 x 8 rows of 4096: 93 us, 6.5 TB/s; eight 106, four 121)
-  int64_t tpb = a.T * parts / (16 * (int64_t)a.num_sms);
-  const int64_t most = a.k > 4096 / kMaxTpb ? 4096 / a.k : kMaxTpb;  // slots and weights: at most 32 KB
-  tpb = tpb < 1 ? 1 : tpb > most ? most : tpb;
-  const dim3 grid((unsigned)((a.T + tpb - 1) / tpb), parts);
-  const size_t smem = (size_t)tpb * a.k * 8;
+  const dim3 grid((unsigned)a.T, column_parts(a.T, nv, 128, a.num_sms));
+  const size_t smem = (size_t)a.k * 8;
   if (vec)
-    expert_combine_kernel<T, O, 8><<<grid, threads, smem, stream>>>(a, (int)tpb);
+    expert_combine_kernel<T, O, 8><<<grid, 128, smem, stream>>>(a);
   else
-    expert_combine_kernel<T, O, 1><<<grid, threads, smem, stream>>>(a, (int)tpb);
+    expert_combine_kernel<T, O, 1><<<grid, 128, smem, stream>>>(a);
 }
 template <typename T, typename O>
 void combine_bwd_typed(const CombineBwdArgs& a, bool vec, cudaStream_t stream) {
+  // 64 threads: 6001 x 6 rows of 2048 take 57.8 us against 61.0 with 128, 1024 x 8 of 4096 27.2 against 29.1, 4096 x 8
+  // of 4096 94.6 (6.0 TB/s) either way; 128 where few tokens leave the GPU idle (8 tokens: 8.7 us a call against 10.7)
+  const int threads = a.T < 512 ? 128 : 64;
   if (vec)
-    expert_combine_bwd_kernel<T, O, 8><<<(unsigned)a.T, 256, 0, stream>>>(a);
+    expert_combine_bwd_kernel<T, O, 8><<<(unsigned)a.T, threads, 0, stream>>>(a);
   else
-    expert_combine_bwd_kernel<T, O, 1><<<(unsigned)a.T, 256, 0, stream>>>(a);
+    expert_combine_bwd_kernel<T, O, 1><<<(unsigned)a.T, threads, 0, stream>>>(a);
 }
 
 }  // namespace
