@@ -115,19 +115,27 @@ __global__ void __launch_bounds__(512) add_rmsnorm_mx_kernel(const NormMxArgs a)
 // Each thread row of the grid (blockIdx.x, threadIdx.y) keeps its columns' sums of dw over the rows it walks;
 // part[blockIdx.x] receives the block's, and norm_dw_kernel adds the blocks in order (the result does not depend
 // on timing).
-// A thread keeps kVpt vectors of a row packed between the two passes, and loads the next row's before it reduces the
-// current one's sums, so that the loads of every resident block are always in flight.  Bound by the instructions
-// of a row's reduction as much as by HBM: two vectors a thread take 56 us for 8192 rows of 4096 (4.8 TB/s), one
-// 70, and rows through a ring of bulk copies 66.
+// Rows come through a ring in shared memory, kDepth - 1 ahead, by asynchronous copies: each thread copies the vectors
+// that it reads itself (kVpt of each operand), so the ring needs no barrier, and both passes over a row read it there.
+// Bound by HBM: 43 us for 8192 rows of 4096 with dres (6.2 TB/s), 48.3 with norm_dw_kernel (55.9 with the next row in
+// registers instead of the ring, and norm_dw_kernel launched after this one).  One vector a thread is slower (twice
+// the reductions), and so are three blocks of 256 threads an SM (80 registers).
 constexpr int kVpt = 2;
+constexpr int kDepth = 3;  // of the ring: two take 53.9 us (norm_dw_kernel after it), three 51.7, four 51.9
+__device__ __forceinline__ void copy16(uint4* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(pm::smem_u32(to)), "l"(__cvta_generic_to_global(from)) : "memory");
+}
 template <typename T>
 __global__ void __launch_bounds__(512, 1) rmsnorm_bwd_kernel(const NormBwdArgs a) {
-  extern __shared__ __align__(16) float sums[];  // [group - 1][n]
+  extern __shared__ __align__(16) uint4 ring[];
+  float* sums = reinterpret_cast<float*>(ring);  // [group - 1][n], at the end
   __shared__ float red[2][2 * kMaxWarps][kMaxWarps];
   const int nv = a.n >> 3, tx = threadIdx.x, ty = threadIdx.y, group = blockDim.y;
   const int64_t step = (int64_t)gridDim.x * group;
+  const int threads = blockDim.x * blockDim.y, tensors = a.dres ? 3 : 2;
+  uint4* slot = ring + ty * blockDim.x + tx;
+  pm::griddep_launch_dependents();  // norm_dw_kernel waits for this grid's end
   float w[kVpt][8], dw[kVpt][8];
-  uint4 sp[kVpt], gp[kVpt], res[kVpt];
 #pragma unroll
   for (int j = 0; j < kVpt; ++j) {
     const int c = tx + j * blockDim.x;
@@ -135,38 +143,45 @@ __global__ void __launch_bounds__(512, 1) rmsnorm_bwd_kernel(const NormBwdArgs a
     for (int i = 0; i < 8; ++i) w[j][i] = dw[j][i] = 0.f;
     if (c < nv) rows::load8<float>(a.w + c * 8, w[j]);
   }
+  int put = 0, take = 0;
   auto fetch = [&](int64_t row) {
+    uint4* to = slot + put * (tensors * kVpt * threads);
 #pragma unroll
     for (int j = 0; j < kVpt; ++j) {
       const int c = tx + j * blockDim.x;
-      res[j] = sp[j] = gp[j] = make_uint4(0, 0, 0, 0);
       if (row < a.rows && c < nv) {
-        sp[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row * a.xs + c * 8);
-        gp[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.dh) + row * a.dhs + c * 8);
-        if (a.dres) res[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.dres) + row * a.drs + c * 8);
+        copy16(to + j * threads, static_cast<const T*>(a.x) + row * a.xs + c * 8);
+        copy16(to + (kVpt + j) * threads, static_cast<const T*>(a.dh) + row * a.dhs + c * 8);
+        if (a.dres) copy16(to + (2 * kVpt + j) * threads, static_cast<const T*>(a.dres) + row * a.drs + c * 8);
       }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    put = put + 1 == kDepth ? 0 : put + 1;
   };
   const float inv_n = 1.f / a.n;
   bool flip = false;
   int64_t row0 = (int64_t)blockIdx.x * group;
-  fetch(row0 + ty);
+#pragma unroll
+  for (int q = 0; q < kDepth - 1; ++q) fetch(row0 + ty + q * step);
   for (; row0 < a.rows; row0 += step) {
     const int64_t row = row0 + ty;
-    float s[kVpt][8], g[kVpt][8], o[kVpt][8];
     float sum[2] = {0.f, 0.f};
+    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
+    const uint4* from = slot + take * (tensors * kVpt * threads);
+    take = take + 1 == kDepth ? 0 : take + 1;
 #pragma unroll
-    for (int j = 0; j < kVpt; ++j) {
-      rows::unpack8<T>(sp[j], s[j]);
-      rows::unpack8<T>(gp[j], g[j]);
-      rows::unpack8<T>(res[j], o[j]);
+    for (int j = 0; j < kVpt; ++j)
+      if (tx + j * blockDim.x < nv) {
+        float s[8], g[8];
+        rows::unpack8<T>(from[j * threads], s);
+        rows::unpack8<T>(from[(kVpt + j) * threads], g);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        sum[0] = fmaf(s[j][i], s[j][i], sum[0]);
-        sum[1] = fmaf(g[j][i] * w[j][i], s[j][i], sum[1]);
+        for (int i = 0; i < 8; ++i) {
+          sum[0] = fmaf(s[i], s[i], sum[0]);
+          sum[1] = fmaf(g[i] * w[j][i], s[i], sum[1]);
+        }
       }
-    }
-    fetch(row + step);
+    fetch(row + (kDepth - 1) * step);
     row_sum<2>(sum, red[flip]);  // two buffers: a slow warp may still read the last group's sums
     flip = !flip;
     const float r = rsqrtf(sum[0] * inv_n + a.eps);
@@ -175,18 +190,24 @@ __global__ void __launch_bounds__(512, 1) rmsnorm_bwd_kernel(const NormBwdArgs a
     for (int j = 0; j < kVpt; ++j) {
       const int c = tx + j * blockDim.x;
       if (row < a.rows && c < nv) {
+        float s[8], g[8], o[8];
+        rows::unpack8<T>(from[j * threads], s);
+        rows::unpack8<T>(from[(kVpt + j) * threads], g);
+        rows::unpack8<T>(a.dres ? from[(2 * kVpt + j) * threads] : make_uint4(0, 0, 0, 0), o);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float t = r * g[j][i];
-          dw[j][i] = fmaf(t, s[j][i], dw[j][i]);
-          o[j][i] = fmaf(-k, s[j][i], fmaf(t, w[j][i], o[j][i]));
+          const float t = r * g[i];
+          dw[j][i] = fmaf(t, s[i], dw[j][i]);
+          o[i] = fmaf(-k, s[i], fmaf(t, w[j][i], o[i]));
         }
-        *reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + row * a.n + c * 8) = rows::pack8<T>(o[j]);
-        if (a.dxf) rows::store8f(a.dxf + row * a.n + c * 8, o[j]);
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + row * a.n + c * 8) = rows::pack8<T>(o);
+        if (a.dxf) rows::store8f(a.dxf + row * a.n + c * 8, o);
       }
     }
   }
   // the block's rows of sums become one, in row order
+  asm volatile("cp.async.wait_group 0;" ::: "memory");  // the ring's memory is free
+  __syncthreads();
   if (ty > 0) {
 #pragma unroll
     for (int j = 0; j < kVpt; ++j) {
@@ -215,6 +236,7 @@ __global__ void __launch_bounds__(512, 1) rmsnorm_bwd_kernel(const NormBwdArgs a
 __global__ void __launch_bounds__(256) norm_dw_kernel(const float* __restrict__ part, int slots, int n,
                                                       float* __restrict__ dw) {
   __shared__ float4 red[64][4];
+  pm::griddep_wait();  // (nothing is read or written before the grids ahead have ended)
   const int c = (blockIdx.x * 4 + threadIdx.x) * 4;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (c < n) {
@@ -299,9 +321,21 @@ void launch_rmsnorm_bwd(const NormBwdArgs& a, int slots, cudaStream_t stream) {
   const dim3 block = norm_block(a.n, kVpt);
   if (slots > 0) {
     auto* fn = a.half ? rmsnorm_bwd_kernel<__half> : rmsnorm_bwd_kernel<__nv_bfloat16>;
-    fn<<<slots, block, (block.y - 1) * a.n * sizeof(float), stream>>>(a);
+    const size_t ring = (size_t)kDepth * (a.dres ? 3 : 2) * kVpt * block.x * block.y * sizeof(uint4);
+    const size_t sums = (block.y - 1) * a.n * sizeof(float), smem = ring > sums ? ring : sums;  // at most 144 KB
+    if (smem > 40 * 1024) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    fn<<<slots, block, smem, stream>>>(a);
   }
-  norm_dw_kernel<<<(a.n + 15) / 16, dim3(4, 64), 0, stream>>>(a.part, slots, a.n, a.dw);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((a.n + 15) / 16);
+  cfg.blockDim = dim3(4, 64);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};  // launched while the rows are still walked (3 us less)
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, norm_dw_kernel, static_cast<const float*>(a.part), slots, a.n, a.dw);
 }
 
 void launch_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t n, void* out, cudaStream_t stream) {
