@@ -44,9 +44,10 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*red)[kMaxWarps]) 
 
 // Thread t of a row owns the 8-column vectors t, t + blockDim.x, ... (VPT of them), so the 4 lanes that share a
 // 32-column group are neighbours.  One group of blockDim.y rows per block: the many resident blocks hide the
-// latency of each other's loads, reductions and stores.
+// latency of each other's loads, reductions and stores.  Four blocks of 512 (32 registers, no spills): 4096 rows of
+// 8192 take 76 us against 81 with the 38 registers of three.
 template <typename T, int VPT>
-__global__ void __launch_bounds__(512) add_rmsnorm_mx_kernel(const NormMxArgs a) {
+__global__ void __launch_bounds__(512, 4) add_rmsnorm_mx_kernel(const NormMxArgs a) {
   __shared__ float red[kMaxWarps][kMaxWarps];
   const int nv = a.n >> 3, tx = threadIdx.x;
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
