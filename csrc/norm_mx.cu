@@ -289,8 +289,8 @@ dim3 norm_block(int n, int vpt) {
   const int ty = tx >= 256 ? 1 : 256 / tx;
   return dim3(tx, ty);
 }
-// Vectors of a thread by width: one up to 4096 columns (73 us, 6.0 TB/s, for 8192 rows of 4096 against 77 with two,
-// 2.7 us against 3.6 for 8 rows: half the serial work of a thread), two beyond (512 threads).
+// Vectors of a thread by width: one up to 4096 columns (2.7 us for 8 rows of 4096 against 3.6 with two, half the serial
+// work of a thread; 27.2 for 4999 rows of 2080 against 29.5; 74 for 8192 of 4096, 5.9 TB/s, against 72), two beyond.
 template <int VPT>
 void launch_fwd(const NormMxArgs& a, cudaStream_t stream) {
   const dim3 block = norm_block(a.n, VPT);
