@@ -492,7 +492,9 @@ struct Gather : Function<Gather> {
 struct Combine : Function<Combine> {
   static Tensor forward(AutogradContext* ctx, const Tensor& y, const OptTensor& weights, const OptTensor& residual,
                         const Tensor& slots, const Tensor& offsets, bool out_f32) {
-    ctx->save_for_backward({y, weights ? *weights : Tensor(), slots, offsets});
+    // without weights no gradient reads the rows
+    ctx->save_for_backward({weights ? y : Tensor(), weights ? *weights : Tensor(), slots, offsets});
+    ctx->saved_data["type"] = static_cast<int64_t>(y.scalar_type());
     ctx->saved_data["res"] = residual.has_value();
     return expert_combine(y, weights, residual, slots, offsets, out_f32);
   }
@@ -504,7 +506,7 @@ struct Combine : Function<Combine> {
     const bool need_dy = ctx->needs_input_grad(0), need_dw = weights.defined() && ctx->needs_input_grad(1);
     Tensor dy, dw;
     if (!weights.defined()) {
-      if (need_dy) dy = std::get<0>(expert_gather(g[0], c10::nullopt, saved[2], saved[3])).to(y.scalar_type());
+      if (need_dy) dy = std::get<0>(expert_gather(g[0], c10::nullopt, saved[2], saved[3])).to(static_cast<torch::ScalarType>(ctx->saved_data["type"].toInt()));
     } else {
       auto [a, b] = expert_combine_backward(g[0], y, weights, saved[2], saved[3], need_dy, need_dw);
       if (a) dy = *a;

@@ -121,7 +121,8 @@ class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, residual, out_dtype, *order):
         ctx.order = ExpertOrder(*order)
-        ctx.save_for_backward(y, weights)
+        ctx.save_for_backward(y if weights is not None else None, weights)  # unweighted: no gradient reads the rows
+        ctx.dtype = y.dtype
         return _combine(y, ctx.order, weights, residual, out_dtype)
 
     @staticmethod
@@ -131,7 +132,7 @@ class _Combine(torch.autograd.Function):
         need = ctx.needs_input_grad
         dy = dw = None
         if weights is None:
-            dy = _gather(dout, ctx.order).to(y.dtype) if need[0] else None
+            dy = _gather(dout, ctx.order).to(ctx.dtype) if need[0] else None
         elif need[0] or need[1]:
             dy, dw = combine_backward(dout, y, ctx.order, weights, need[0], need[1])
         return (dy, dw, dout if need[2] else None) + (None,) * 4

@@ -727,3 +727,45 @@ def test_norm_inplace_is_seen_and_checked(cuda):
         b = a.clone()
         new, *_ = fused.add_rmsnorm_mx(a, w, 1e-6, d, inplace=True)
         assert torch.equal(new, fused.add_rmsnorm_mx(b, w, 1e-6, d)[0])
+
+
+def test_exchange_and_norm_gradient_repeat_in_a_graph(cuda):
+    """Calls whose second kernel starts ahead of the first one's end, captured and replayed on changing inputs."""
+    g = gen(51)
+    T, k, E, H = 700, 4, 16, 544
+    ids = torch.randint(-1, E, (T, k), device="cuda", generator=g)
+    x, dh = randn(g, T, H, dtype=BF16), randn(g, T, H, dtype=BF16)
+    weights, w = torch.rand(T, k, device="cuda", generator=g), 1 + 0.1 * randn(g, H)
+
+    def run():
+        order = dispatch.expert_order(ids, E)
+        out = dispatch.combine(dispatch.gather(x, order), order, weights)
+        return (*order, out, *dispatch.combine_backward(dh, dispatch.gather(dh, order), order, weights),
+                *fused.add_rmsnorm_backward(dh, x, w, 1e-6, out))
+
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for _ in range(20):
+        ids.copy_(torch.randint(-1, E, (T, k), device="cuda", generator=g))
+        x.copy_(randn(g, T, H, dtype=BF16))
+        graph.replay()
+        for a, b in zip(got, run()):
+            assert torch.equal(a, b)
+    check_errors(cuda)
+
+
+def test_unweighted_combine_keeps_no_rows(cuda):
+    """Without weights the gradient does not read the rows: they may be written over before it runs."""
+    g = gen(61)
+    order = routed(30, 2, 4, 0.2, 7)
+    y = randn(g, 60, 40, dtype=F16)
+    leaf = y.clone().requires_grad_(True)
+    rows = leaf * 1
+    out = dispatch.combine(rows, order, out_dtype=F32)
+    with torch.no_grad():
+        rows.zero_()
+    v = randn(g, 30, 40)
+    got, = torch.autograd.grad(out, leaf, v)
+    assert got.dtype == F16 and torch.equal(got, dispatch.gather(v, order).half())
