@@ -6,7 +6,8 @@
 //   kGradW     dW_e = dz_e^T x_e         (zero for an expert without rows)
 //
 // Expert e owns rows offsets[e] .. offsets[e + 1]; the offsets are read on the device, so no call waits for
-// the host.  Rows past offsets[E] give zero rows (kForward, kGradX) and are not read (kGradW).
+// the host.  Rows before offsets[0] (a table of some of a larger table's experts) and past offsets[E] give zero rows
+// (kForward, kGradX) and are not read (kGradW).
 #include <cuda.h>
 
 #include "launchers.h"
@@ -24,15 +25,19 @@ enum Mode { kForward = 0, kGradX = 1, kGradW = 2 };
 __device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
 __device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.f + __expf(-g)); }
 
-// off[0 .. E]: offsets clamped to 0 = off[0] <= off[e] <= off[e + 1] <= P (a wrong table must not reach memory);
-// start[0 .. E + 1]: first tile of each expert, for tiles(rows of e, e) tiles each; "expert" E is the rows past
-// the last one.  Called by one warp.
+// off[0 .. E]: the running maximum of the offsets, clamped to 0 .. P (a wrong table must not reach memory);
+// start[0 .. E + 2]: first tile of each expert, for tiles(rows of e, e) tiles each; "expert" E is the rows past the
+// last one and "expert" E + 1 those before the first.  Called by one warp.
+__device__ __forceinline__ int first_row(const ExpertMmArgs& a, const int32_t* off, int e) { return e <= a.E ? off[e] : 0; }
+__device__ __forceinline__ int row_count(const ExpertMmArgs& a, const int32_t* off, int e) {
+  return e < a.E ? off[e + 1] - off[e] : e == a.E ? a.P - off[e] : off[0];
+}
 template <typename Tiles>
 __device__ __forceinline__ void tile_table(const ExpertMmArgs& a, int32_t* off, int32_t* start, int lane, Tiles tiles) {
   int carry_off = 0, carry_t = 0;
   for (int e0 = 0; e0 <= a.E; e0 += 32) {
     const int e = e0 + lane;
-    int o = e > 0 && e <= a.E ? min(max(a.offsets[e], 0), a.P) : 0;
+    int o = e <= a.E ? min(max(a.offsets[e], 0), a.P) : 0;
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, o, s);
@@ -43,15 +48,15 @@ __device__ __forceinline__ void tile_table(const ExpertMmArgs& a, int32_t* off, 
     carry_off = __shfl_sync(0xffffffffu, o, 31);
   }
   __syncwarp();
-  for (int e0 = 0; e0 <= a.E; e0 += 32) {
+  for (int e0 = 0; e0 <= a.E + 1; e0 += 32) {
     const int e = e0 + lane;
-    int inc = e <= a.E ? tiles((e < a.E ? off[e + 1] : a.P) - off[e], e) : 0;
+    int inc = e <= a.E + 1 ? tiles(row_count(a, off, e), e) : 0;
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, inc, s);
       if (lane >= s) inc += u;
     }
-    if (e <= a.E) start[e + 1] = carry_t + inc;
+    if (e <= a.E + 1) start[e + 1] = carry_t + inc;
     carry_t += __shfl_sync(0xffffffffu, inc, 31);
   }
   if (lane == 0) start[0] = 0;
@@ -112,9 +117,9 @@ struct PairWalker {
   __device__ bool next(PairTile& k) {
     t += gridDim.x >> 1;
     const int E = a.E;
-    if (t >= start[E + 1]) return false;
+    if (t >= start[E + 2]) return false;
     while (t >= start[e + 1]) ++e;
-    const int rel = t - start[e], first = off[e], rows = (e < E ? off[e + 1] : a.P) - first;
+    const int rel = t - start[e], first = first_row(a, off, e), rows = row_count(a, off, e);
     const int tn = MODE == kGradW ? a.tiles_n : (rows + 255) / 256;
     const int band = rel / (kBand * a.tiles_m), in = rel - band * kBand * a.tiles_m, h = min(kBand, tn - band * kBand);
     k.e = e;
@@ -473,18 +478,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
 
 // ----------------------------------------------------------------------------- SwiGLU gradient
 // da = gradient of silu(g) u; z = [g | u] rows: dg = da u s (1 + g (1 - s)), du = da g s with s = sigmoid(g).
-// Rows past offsets[E] are zero.  Memory bound: 6 bytes read and 4 written per value of da; a block per row (58 us
+// Rows before offsets[0] and past offsets[E] are zero.  Memory bound: 6 bytes read and 4 written per value of da; a block per row (58 us
 // for 16384 x 2048, 5.8 TB/s; walking blocks 61 us).
 template <typename T>
 __global__ void __launch_bounds__(256) swiglu_bwd_kernel(const T* __restrict__ da, int64_t das,
                                                          const T* __restrict__ z, int64_t zs, T* __restrict__ dz,
                                                          int64_t P, int I, const int32_t* __restrict__ offsets, int E) {
   const int nv = I / 8;
-  const int64_t total = offsets[E];
   const int64_t row = blockIdx.x;
+  const bool owned = row >= offsets[0] && row < offsets[E];
   for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < nv; c += gridDim.y * blockDim.x) {
     float d[8], g[8], u[8];
-    if (row < total) {
+    if (owned) {
       rows::load8<T>(da + row * das + c * 8, d);
       rows::load8<T>(z + row * zs + c * 8, g);
       rows::load8<T>(z + row * zs + I + c * 8, u);
@@ -509,7 +514,7 @@ constexpr int kMaxSmem = 232448;
 template <typename T, int MODE, bool GATED>
 int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb64, const CUtensorMap& tb32, const ExpertMmArgs& a,
                 cudaStream_t stream) {
-  const int smem = (int)(Pair::kFixed + (2 * a.E + 3) * sizeof(int32_t));
+  const int smem = (int)(Pair::kFixed + (2 * a.E + 4) * sizeof(int32_t));
   if (smem > kMaxSmem) return -2;
   auto* fn = expert_pair_kernel<T, MODE, GATED>;
   cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);

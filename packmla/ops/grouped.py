@@ -2,8 +2,9 @@
 
 Rows are sorted by expert (`ops/dispatch.py`): expert e owns rows offsets[e] .. offsets[e + 1] of x, and its
 weight is w[e] [N, K] (K contiguous, the convention of the model's `w13` = [gate rows | up rows] and `w2`).
-The offsets stay on the device.  Rows past offsets[E] give zero rows.  CUDA: csrc/expert_mm.cu (tcgen05, BF16 or
-FP16 operands, fp32 accumulators, one rounding); CPU tensors: the same products in fp32.
+The offsets ascend and stay on the device.  Rows before offsets[0] and past offsets[E] give zero rows, so a slice
+offsets[a : b + 1] with w[a : b] computes some of a larger table's experts.  CUDA: csrc/expert_mm.cu (tcgen05, BF16
+or FP16 operands, fp32 accumulators, one rounding); CPU tensors: the same products in fp32.
 """
 from __future__ import annotations
 
@@ -66,8 +67,8 @@ def expert_linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, o
 
 
 def swiglu_backward(dy: torch.Tensor, pre: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
-    """Gradient [P, N] of silu(gate) * up with respect to pre = [gate | up], from dy [P, N / 2]; rows past
-    offsets[E] are zero."""
+    """Gradient [P, N] of silu(gate) * up with respect to pre = [gate | up], from dy [P, N / 2]; rows
+    before offsets[0] and past offsets[E] are zero."""
     if pre.dim() != 2 or pre.shape[1] % 16 or pre.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("pre must be a BF16 or FP16 [rows, n] tensor, n a multiple of 16")
     if dy.shape != (pre.shape[0], pre.shape[1] // 2) or dy.dtype != pre.dtype:
@@ -75,7 +76,9 @@ def swiglu_backward(dy: torch.Tensor, pre: torch.Tensor, offsets: torch.Tensor) 
     if pre.is_cuda:
         return ext().swiglu_backward(dy, pre, offsets)
     dz = _silu_grad(pre, dy)
-    dz[_spans(offsets, pre.shape[0])[-1][1]:] = 0
+    spans = _spans(offsets, pre.shape[0])
+    dz[:spans[0][0]] = 0
+    dz[spans[-1][1]:] = 0
     return dz.to(pre.dtype)
 
 

@@ -1,0 +1,30 @@
+"""Expert block operators on CPU tensors at the edges of their contracts."""
+import pytest
+import torch
+
+import expert_block_reference as ref
+from expert_block_reference import ACC, F64
+from packmla.ops import grouped
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.mark.parametrize("table", [[4, 10], [3, 3, 8, 11], [12, 12]])
+def test_rows_before_the_first_expert(table):
+    """A table that starts past row 0 (some experts of a larger one): the rows before it belong to nobody."""
+    g = torch.Generator().manual_seed(len(table))
+    P, E, K, N = 12, len(table) - 1, 24, 32
+    offsets = torch.tensor(table, dtype=torch.int32)
+    x, dy, w = (torch.randn(*s, generator=g).to(BF16) for s in ((P, K), (P, N), (E, N, K)))
+    nobody = torch.ones(P, dtype=torch.bool)
+    nobody[table[0]:table[-1]] = False
+    x[nobody], dy[nobody] = float("nan"), float("inf")
+    z, s = ref.linear(x, w, offsets)
+    ref.check(grouped.expert_linear(x, w, offsets), z, s * ACC * K, "y")
+    dx, dw = grouped.expert_linear_backward(dy, x, w, offsets)
+    rdx, s = ref.linear(dy, w.transpose(1, 2), offsets)
+    ref.check(dx, rdx, s * ACC * N, "dx")
+    for e, (a, b) in enumerate(zip(table, table[1:])):
+        ref.check(dw[e], dy[a:b].to(F64).T @ x[a:b].to(F64), (dy[a:b].to(F64).abs().T @ x[a:b].to(F64).abs()) * ACC * P, "dw")
+    assert (grouped.expert_linear(x, w, offsets, activation="swiglu")[nobody] == 0).all()
+    assert (grouped.swiglu_backward(dy[:, :N // 2], dy, offsets)[nobody] == 0).all()

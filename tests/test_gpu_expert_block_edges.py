@@ -1,0 +1,75 @@
+"""Expert block kernels at the edges of their contracts, against 64-bit references."""
+import pytest
+import torch
+
+import expert_block_reference as ref
+from expert_block_reference import ACC, F64
+from packmla.ops import check_errors, grouped
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape, dtype=F32, scale=1.0):
+    return (torch.randn(*shape, device="cuda", generator=g) * scale).to(dtype)
+
+
+# ------------------------------------------------------------------------------------------------ tables
+def check_products(dy, x, w, offsets, rows):
+    """Products and gradients against the reference on `rows`, the table they have to follow."""
+    N, K = w.shape[1:]
+    z, s = ref.linear(x, w, rows)
+    ref.check(grouped.expert_linear(x, w, offsets), z, s * ACC * K, "y")
+    dx, dw = grouped.expert_linear_backward(dy, x, w, offsets)
+    rdx, s = ref.linear(dy, w.transpose(1, 2), rows)
+    ref.check(dx, rdx, s * ACC * N, "dx")
+    for e, (a, b) in enumerate(zip(rows.tolist(), rows.tolist()[1:])):
+        d, v = dy[a:b].to(F64), x[a:b].to(F64)
+        ref.check(dw[e], d.T @ v, (d.abs().T @ v.abs()) * ACC * max(1, b - a), f"dw[{e}]")
+    check_errors(x.device)
+
+
+TABLES = [[4, 10], [1, 1, 340], [130, 130, 300, 333], [300, 300, 300], [7, 263, 270, 300], [340, 340]]
+
+
+@pytest.mark.parametrize("K,N,dtype", [(64, 32, BF16), (200, 528, F16)])
+@pytest.mark.parametrize("table", TABLES)
+def test_rows_before_the_first_expert(cuda, table, K, N, dtype):
+    """A table that starts past row 0 (some experts of a larger one): the rows before it belong to nobody."""
+    P, E = 340, len(table) - 1
+    g = gen(len(table) + K)
+    offsets = torch.tensor(table, dtype=torch.int32, device="cuda")
+    x, dy = randn(g, P, K, dtype=dtype), randn(g, P, N, dtype=dtype)
+    w = randn(g, E, N, K, dtype=dtype, scale=K ** -0.5)
+    nobody = torch.ones(P, dtype=torch.bool, device="cuda")
+    nobody[table[0]:table[-1]] = False
+    x[nobody] = float("nan")
+    dy[nobody] = float("inf")
+    check_products(dy, x, w, offsets, offsets)
+    y = grouped.expert_linear(x, w, offsets, activation="swiglu")
+    assert (y[nobody] == 0).all() and y.isfinite().all()
+    assert (grouped.swiglu_backward(dy[:, :N // 2], dy, offsets)[nobody] == 0).all()
+
+
+def test_experts_of_a_larger_table(cuda):
+    """offsets[a : b + 1] is the table of experts a .. b: their rows give what the whole table gives, with gradients."""
+    g = gen(3)
+    table = torch.tensor([0, 40, 300, 300, 420, 500], dtype=torch.int32, device="cuda")
+    x, w = randn(g, 500, 96, dtype=BF16), randn(g, 5, 64, 96, dtype=BF16, scale=0.1)
+    part = table[1:5]
+    for activation in (None, "swiglu"):
+        whole = grouped.expert_linear(x, w, table, activation)
+        xr, wr = x.clone().requires_grad_(True), w[1:4].clone().requires_grad_(True)
+        y = grouped.expert_linear(xr, wr, part, activation)
+        assert torch.equal(y[40:420], whole[40:420])
+        assert (y[:40] == 0).all() and (y[420:] == 0).all()
+        dx, dw = torch.autograd.grad(y, [xr, wr], torch.ones_like(y))
+        assert (dx[:40] == 0).all() and (dx[420:] == 0).all()
+        full = [x.clone().requires_grad_(True), w.clone().requires_grad_(True)]
+        want = torch.autograd.grad(grouped.expert_linear(*full, table, activation), full, torch.ones_like(whole))
+        assert torch.equal(dx[40:420], want[0][40:420]) and torch.equal(dw, want[1][1:4])
+    check_errors(cuda)
