@@ -28,6 +28,7 @@ namespace cg = cooperative_groups;
 // rows in the same order.  Latency bound: a lane's first kHeld ids and its peers of equal expert stay in
 // registers for both passes, the ids loaded together, and each CTA pushes its counts into the others' shared
 // memory, so that after the cluster barrier all reads are local.
+constexpr int kOrderSmem = 200 * 1024;  // counters of a CTA at most
 constexpr int kHeld = 8;  // ids of a lane held in registers (8 x 32 lanes x 16 warps x 16 CTAs = 65536 pairs)
 
 template <typename Id>
@@ -446,7 +447,7 @@ int launch_expert_order(const void* ids, bool wide, int64_t n, int64_t base, int
   while (cluster < 16 && (int64_t)cluster * 512 < n) cluster *= 2;
   int warps = (int)((n + 32 * cluster - 1) / (32 * cluster));
   warps = warps < 4 ? 4 : warps > 16 ? 16 : warps;
-  const int counters = 200 * 1024 / 4 / E;  // shared memory: (warps + CTAs) counters of every expert
+  const int counters = kOrderSmem / 4 / E;  // shared memory: (warps + CTAs) counters of every expert
   while (cluster > 1 && counters - cluster < 8) cluster /= 2;
   warps = warps > counters - cluster ? counters - cluster : warps;
   if (warps < 1) return -1;
@@ -463,7 +464,9 @@ int launch_expert_order(const void* ids, bool wide, int64_t n, int64_t base, int
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   auto go = [&](auto* fn, auto* p) {
-    if (smem > 40 * 1024) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // the limit is the kernel's, not this launch's: always the largest, or a smaller launch of another host thread
+    // could lower it before this one
+    if (smem > 40 * 1024) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kOrderSmem);
     if (cluster > 8) cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     return (int)cudaLaunchKernelEx(&cfg, fn, p, (int)n, base, E, offsets, slots, pairs);
   };

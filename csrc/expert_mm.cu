@@ -517,7 +517,9 @@ int launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap&
   const int smem = (int)(Pair::kFixed + (2 * a.E + 4) * sizeof(int32_t));
   if (smem > kMaxSmem) return -2;
   auto* fn = expert_pair_kernel<T, MODE, GATED>;
-  cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  // the limit is the kernel's, not this launch's: always the largest, or a launch of another host thread with fewer
+  // experts could lower it before this one
+  cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
   fn<<<a.num_sms / 2 * 2, pair_threads(MODE), smem, stream>>>(ta, tb, tb64, tb32, a);
   return 0;
 }

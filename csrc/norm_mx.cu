@@ -323,8 +323,11 @@ void launch_rmsnorm_bwd(const NormBwdArgs& a, int slots, cudaStream_t stream) {
   if (slots > 0) {
     auto* fn = a.half ? rmsnorm_bwd_kernel<__half> : rmsnorm_bwd_kernel<__nv_bfloat16>;
     const size_t ring = (size_t)kDepth * (a.dres ? 3 : 2) * kVpt * block.x * block.y * sizeof(uint4);
-    const size_t sums = (block.y - 1) * a.n * sizeof(float), smem = ring > sums ? ring : sums;  // at most 144 KB
-    if (smem > 40 * 1024) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const size_t sums = (block.y - 1) * a.n * sizeof(float), smem = ring > sums ? ring : sums;
+    // the limit is the kernel's, not this launch's: always the largest (a ring of 512 threads and three operands), or a
+    // smaller launch of another host thread could lower it before this one
+    constexpr int most = kDepth * 3 * kVpt * 512 * (int)sizeof(uint4);
+    if (smem > 40 * 1024) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     fn<<<slots, block, smem, stream>>>(a);
   }
   cudaLaunchConfig_t cfg{};

@@ -1,10 +1,13 @@
 """Expert block kernels at the edges of their contracts, against 64-bit references."""
+import sys
+from concurrent.futures import ThreadPoolExecutor
+
 import pytest
 import torch
 
 import expert_block_reference as ref
 from expert_block_reference import ACC, F64
-from packmla.ops import check_errors, grouped
+from packmla.ops import check_errors, dispatch, fused, grouped
 
 pytestmark = pytest.mark.gpu
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -72,4 +75,41 @@ def test_experts_of_a_larger_table(cuda):
         full = [x.clone().requires_grad_(True), w.clone().requires_grad_(True)]
         want = torch.autograd.grad(grouped.expert_linear(*full, table, activation), full, torch.ones_like(whole))
         assert torch.equal(dx[40:420], want[0][40:420]) and torch.equal(dw, want[1][1:4])
+    check_errors(cuda)
+
+
+# ------------------------------------------------------------------------------------------------ host threads
+def together(*calls, times=20000):
+    """Every call from a thread and on a stream of its own, many times and closely interleaved; raises what any raised."""
+    def loop(call):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(times):
+                call()
+            torch.cuda.current_stream().synchronize()
+
+    torch.cuda.synchronize()
+    interval = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    try:
+        with ThreadPoolExecutor(len(calls)) as pool:
+            for done in [pool.submit(loop, c) for c in calls]:
+                done.result()
+    finally:
+        sys.setswitchinterval(interval)
+
+
+def test_calls_of_two_threads_with_other_sizes(cuda):
+    """A launch's shared memory limit belongs to the kernel, not to the call: a smaller call of another thread must
+    not lower it between the larger one's request and its launch."""
+    ids = torch.zeros(4096, 8, dtype=torch.int32, device="cuda")
+    together(lambda: dispatch.expert_order(ids[:64], 4000), lambda: dispatch.expert_order(ids[:512], 500))
+    g = gen(1)
+    wide, narrow = randn(g, 4, 8192, dtype=BF16), randn(g, 4, 4096, dtype=BF16)
+    w = torch.ones(8192, device="cuda")
+    together(lambda: fused.add_rmsnorm_backward(wide, wide, w, 1e-6, wide),
+             lambda: fused.add_rmsnorm_backward(narrow, narrow, w[:4096], 1e-6))
+    x = randn(g, 8, 8, dtype=BF16)
+    many, one = torch.zeros(1024, 8, 8, device="cuda", dtype=BF16), torch.zeros(1, 8, 8, device="cuda", dtype=BF16)
+    table = torch.zeros(1025, device="cuda", dtype=torch.int32)
+    together(lambda: grouped.expert_linear(x, many, table), lambda: grouped.expert_linear(x, one, table[:2]))
     check_errors(cuda)
