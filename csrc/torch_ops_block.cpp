@@ -1,7 +1,6 @@
 // Torch-facing wrappers of the mixture-of-experts block operators (norm_mx.cu, expert_dispatch.cu,
 // expert_mm.cu): argument validation, output allocation, then the plain launchers.
 #include <torch/extension.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -77,6 +76,30 @@ void check_weight(const Tensor& like, const Tensor& w, int64_t n) {
   TORCH_CHECK(w.scalar_type() == torch::kFloat32 && w.dim() == 1 && w.size(0) == n && w.is_contiguous() && on16(w),
               "w must be contiguous fp32 [", num(n), "]");
 }
+// Memory that rows of x and of t share: kNo and kYes are exact.
+enum class Shared { kNo, kYes, kUnknown };
+Shared shared_rows(const Tensor& x, const Tensor& t) {
+  if (x.numel() == 0 || t.numel() == 0) return Shared::kNo;
+  const int64_t xb = x.size(1) * x.element_size(), tb = t.size(1) * t.element_size();
+  const int64_t step = row_stride(x) * x.element_size(), tstep = row_stride(t) * t.element_size();
+  const int64_t apart = reinterpret_cast<intptr_t>(t.data_ptr()) - reinterpret_cast<intptr_t>(x.data_ptr());
+  if (apart >= (x.size(0) - 1) * step + xb || -apart >= (t.size(0) - 1) * tstep + tb) return Shared::kNo;
+  if (x.size(0) == 1 && t.size(0) == 1) return Shared::kYes;
+  if (step != tstep || step < xb || step < tb) return Shared::kUnknown;
+  // rows of one step: t's lie `at` bytes into x's period, between x's columns or not
+  const int64_t at = (apart % step + step) % step;
+  return at >= xb && at + tb <= step ? Shared::kNo : Shared::kYes;
+}
+// An operand of a call that writes over x, as rows that no thread can find written by another: t itself if it is x
+// or shares no memory with it, a copy where the strides do not tell.
+Tensor beside(const Tensor& x, const Tensor& t, const char* name) {
+  if (t.data_ptr() == x.data_ptr() && t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes() && row_stride(t) == row_stride(x))
+    return t;
+  const Shared s = shared_rows(x, t.dim() == 1 ? t.unsqueeze(0) : t);
+  TORCH_CHECK(s != Shared::kYes, "add_rmsnorm_mx: ", name, " and the x that is written over overlap in part");
+  return s == Shared::kNo ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
 void check_norm(const Tensor& x, const char* op) {
   TORCH_CHECK(x.is_cuda() && x.dim() == 2 && is16(x), op, ": x must be a CUDA BF16 or FP16 [rows, n] tensor");
   TORCH_CHECK(x.size(1) >= 32 && x.size(1) % 32 == 0 && x.size(1) <= 8192, op,
@@ -85,25 +108,27 @@ void check_norm(const Tensor& x, const char* op) {
 }  // namespace
 
 // -> (stream, codes, scales, h or None); stream is x itself without addends or in place
-std::tuple<Tensor, Tensor, Tensor, OptTensor> add_rmsnorm_mx(const Tensor& x_in, const Tensor& w, double eps,
+std::tuple<Tensor, Tensor, Tensor, OptTensor> add_rmsnorm_mx(const Tensor& x_in, const Tensor& w_in, double eps,
                                                              const OptTensor& d_in, const OptTensor& df_in, bool inplace,
                                                              bool return_h) {
   check_norm(x_in, "add_rmsnorm_mx");
   const Tensor x = inplace ? x_in : rows16(x_in);
-  const OptTensor d = rows16(d_in), df = rows16(df_in);
+  OptTensor d = rows16(d_in), df = rows16(df_in);
+  Tensor w = w_in;
   const int64_t rows = x.size(0), n = x.size(1);
   check_rows16(x, x, rows, n, x.scalar_type(), "x");
   check_weight(x, w, n);
   if (d) check_rows16(x, *d, rows, n, x.scalar_type(), "d");
   if (df) check_rows16(x, *df, rows, n, torch::kFloat32, "dfp32");
   const bool add = d || df;
+  const c10::cuda::CUDAGuard g(x.device());
   if (inplace && add) {
     TORCH_CHECK(rows <= 1 || row_stride(x) >= n, "add_rmsnorm_mx: inplace needs rows apart from one another");
-    TORCH_CHECK(!d_in || at::get_overlap_status(x, *d_in) != at::MemOverlapStatus::Partial,
-                "add_rmsnorm_mx: d and the x that is written over overlap in part");
+    if (d) d = beside(x, *d, "d");
+    if (df) df = beside(x, *df, "dfp32");
+    w = beside(x, w, "w");
     x.unsafeGetTensorImpl()->bump_version();  // a gradient that saved x's old values must not use the new ones
   }
-  const c10::cuda::CUDAGuard g(x.device());
   Tensor s = add && !inplace ? make({rows, n}, x) : x_in;
   const Tensor mx = make({rows * n + rows * (n / 32)}, x, torch::kUInt8);
   Tensor codes = part_of(mx, 0, {rows, n}, torch::kUInt8);

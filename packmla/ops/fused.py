@@ -192,7 +192,8 @@ def add_rmsnorm_mx(x: torch.Tensor, w: torch.Tensor, eps: float, d: torch.Tensor
                    dfp32: torch.Tensor | None = None, inplace: bool = False, return_h: bool = False):
     """Residual add + RMSNorm with MXFP8 rows out: (x_new, codes, scales, h).
 
-    x_new = x + d + dfp32 in x's type (x itself without an addend; written over x with `inplace`);
+    x_new = x + d + dfp32 in x's type (x itself without an addend; written over x with `inplace`,
+    where d may be x and every other operand has to lie apart from x);
     h = x_new * rsqrt(mean(x_new^2) + eps) * w in fp32; codes [T, n] are the E4M3 codes of h (uint8) and scales
     [T, n / 32] its UE8M0 scale bytes, one per 32 columns; with `return_h`, h rounded to x's type (the router's and
     the shared expert's input), else None.  x, d: BF16 or FP16 [T, n], n a multiple of 32 up to 8192; w fp32 [n].

@@ -113,3 +113,62 @@ def test_calls_of_two_threads_with_other_sizes(cuda):
     table = torch.zeros(1025, device="cuda", dtype=torch.int32)
     together(lambda: grouped.expert_linear(x, many, table), lambda: grouped.expert_linear(x, one, table[:2]))
     check_errors(cuda)
+
+
+# ------------------------------------------------------------------------------------------------ in place
+def test_inplace_norm_and_operands_in_its_memory(cuda):
+    """Rows of a wider buffer: addends in other columns or rows of it are read, ones that x writes over are refused, and
+    where the strides do not tell, the addend is copied first."""
+    g = gen(5)
+    w = 1 + 0.1 * randn(g, 64)
+
+    def both(make):
+        """make(buffer) -> x, d, df, w: in place against the same sums on copies."""
+        buf = randn(g, 40, 256, dtype=BF16)
+        want = fused.add_rmsnorm_mx(*call_args(*(t.clone() if t is not None else None for t in make(buf))))
+        x, *rest = make(buf)
+        keep = buf.clone()
+        new, codes, scales, _ = fused.add_rmsnorm_mx(*call_args(x, *rest), inplace=True)
+        assert new.data_ptr() == x.data_ptr()
+        assert torch.equal(x, want[0]) and torch.equal(codes, want[1]) and torch.equal(scales, want[2])
+        changed = buf != keep
+        x.fill_(7)
+        keep[buf == 7] = 7
+        assert not (changed & (keep != 7)).any()  # nothing but x was written
+
+    def call_args(x, d, df, weight):
+        return x, weight, 1e-6, d, df
+
+    def floats(t):  # the same memory as fp32 rows
+        return t.view(F32)
+
+    both(lambda b: (b[:, :64], b[:, 64:128], None, w))
+    both(lambda b: (b[::2, :64], b[1::2, :64], None, w))
+    both(lambda b: (b[:, 64:128], b[:, :64], floats(b)[:, 64:], w))
+    both(lambda b: (b[:20, 8:72], b[20:, 8:72], floats(b)[20:, 64:], w))
+    both(lambda b: (b[:10, :64], b[::4, 128:192], None, w))       # other steps: copied
+    both(lambda b: (b[::4, :64], b[:10, 128:192], None, w))
+    both(lambda b: (b[:, :64], b[:, 64:128], None, floats(b)[3, 64:]))
+    both(lambda b: (b[3:4, :64], b[3:4, 64:128], floats(b)[3:4, 64:], w))
+
+    buf = randn(g, 40, 256, dtype=BF16)
+    keep = buf.clone()
+    x = buf[1:-1, :64]
+    for d in (buf[:-2, :64], buf[2:, :64], buf[1:-1, 32:96], buf[2:, 56:120], buf[1:-1, 8:72]):
+        with pytest.raises(RuntimeError, match="overlap"):
+            fused.add_rmsnorm_mx(x, w, 1e-6, d, inplace=True)
+    with pytest.raises(RuntimeError, match="overlap"):
+        fused.add_rmsnorm_mx(x, w, 1e-6, None, floats(buf)[1:-1, :64], inplace=True)
+    with pytest.raises(RuntimeError, match="overlap"):
+        fused.add_rmsnorm_mx(x, w, 1e-6, None, floats(buf)[:-2, 16:80], inplace=True)
+    with pytest.raises(RuntimeError, match="overlap"):
+        fused.add_rmsnorm_mx(x[:1], floats(buf)[1, 16:80], 1e-6, x[:1], inplace=True)
+    with pytest.raises(RuntimeError, match="overlap"):
+        fused.add_rmsnorm_mx(x[:1], w, 1e-6, buf[1:2, 8:72], inplace=True)
+    wrap = torch.as_strided(buf, (30, 64), (256, 1), 256 + 224)  # columns 224 .. 287: the next row's first 32
+    with pytest.raises(RuntimeError, match="overlap"):
+        fused.add_rmsnorm_mx(buf[1:31, :64], w, 1e-6, wrap, inplace=True)
+    assert torch.equal(buf, keep)
+    want = fused.add_rmsnorm_mx(x.clone(), w, 1e-6, x.clone())
+    new, codes, *_ = fused.add_rmsnorm_mx(x, w, 1e-6, x, inplace=True)  # x on itself
+    assert torch.equal(new, want[0]) and torch.equal(codes, want[1])
