@@ -41,6 +41,18 @@ std::string num(int64_t v) { return std::to_string(v); }
 // Rows of adjacent elements: a column of one element may report any stride.
 bool dense_rows(const Tensor& t) { return t.numel() == 0 || t.size(1) == 1 || t.stride(1) == 1; }
 
+// The operators have no forward-mode derivative: a tangent is refused, where the bare kernels would drop it.
+void check_tangent(const Tensor& t) {
+  TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "the expert block operators have no forward-mode derivative");
+}
+void check_tangent(const OptTensor& t) {
+  if (t) check_tangent(*t);
+}
+template <typename... T>
+void check_tangents(const T&... t) {
+  (check_tangent(t), ...);
+}
+
 void check_device(const Tensor& like, const Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", like.device());
 }
@@ -112,6 +124,7 @@ std::tuple<Tensor, Tensor, Tensor, OptTensor> add_rmsnorm_mx(const Tensor& x_in,
                                                              const OptTensor& d_in, const OptTensor& df_in, bool inplace,
                                                              bool return_h) {
   check_norm(x_in, "add_rmsnorm_mx");
+  check_tangents(x_in, w_in, d_in, df_in);
   const Tensor x = inplace ? x_in : rows16(x_in);
   OptTensor d = rows16(d_in), df = rows16(df_in);
   Tensor w = w_in;
@@ -158,6 +171,7 @@ std::tuple<Tensor, Tensor, Tensor, OptTensor> add_rmsnorm_mx(const Tensor& x_in,
 std::tuple<Tensor, Tensor, OptTensor> rmsnorm_backward(const Tensor& dh_in, const Tensor& x_in, const Tensor& w,
                                                        double eps, const OptTensor& dres_in, bool fp32_dx) {
   check_norm(x_in, "add_rmsnorm_backward");
+  check_tangents(dh_in, x_in, w, dres_in);
   const Tensor x = rows16(x_in), dh = rows16(dh_in);
   const OptTensor dres = rows16(dres_in);
   const int64_t rows = x.size(0), n = x.size(1);
@@ -242,6 +256,7 @@ void check_order(const Tensor& like, const Tensor& offsets, const Tensor& slots)
 // x [T, width] (and scales [T, ...], uint8) -> the same for the sorted rows
 std::tuple<Tensor, OptTensor> expert_gather(const Tensor& x_in, const OptTensor& scales_in, const Tensor& slots,
                                             const Tensor& offsets) {
+  check_tangents(x_in);
   const Tensor x = packed_rows(x_in);
   const OptTensor scales = packed_rows(scales_in);
   TORCH_CHECK(x.is_cuda() && x.dim() == 2, "gather: x must be a CUDA [tokens, width] tensor");
@@ -286,6 +301,7 @@ bool wide(const Tensor& t) { return t.size(1) % 8 == 0 && on16(t) && row_stride(
 
 Tensor expert_combine(const Tensor& y_in, const OptTensor& weights_in, const OptTensor& residual_in,
                       const Tensor& slots, const Tensor& offsets, bool out_f32) {
+  check_tangents(y_in, weights_in, residual_in);
   const Tensor y = packed_rows(y_in);
   const OptTensor weights = packed_rows(weights_in), residual = packed_rows(residual_in);
   const int type = row_type(y, "combine");
@@ -317,6 +333,7 @@ Tensor expert_combine(const Tensor& y_in, const OptTensor& weights_in, const Opt
 std::tuple<OptTensor, OptTensor> expert_combine_backward(const Tensor& dout_in, const Tensor& y_in,
                                                          const Tensor& weights_in, const Tensor& slots,
                                                          const Tensor& offsets, bool need_dy, bool need_dw) {
+  check_tangents(dout_in, y_in, weights_in);
   const Tensor dout = packed_rows(dout_in), y = packed_rows(y_in), weights = packed_rows(weights_in);
   const int type = row_type(y, "combine_backward");
   check_order(y, offsets, slots);
@@ -388,6 +405,7 @@ void run_mm(int mode, const ExpertMmCall& c) {
 std::tuple<Tensor, OptTensor> expert_mm(const Tensor& x_in, const Tensor& w, const Tensor& offsets, bool gated,
                                         bool save_pre, const Tensor& err) {
   check_mm(w, offsets, err, "expert_linear");
+  check_tangents(x_in, w);
   const Tensor x = rows16(x_in);
   const int64_t P = x.size(0), N = w.size(1), K = w.size(2);
   check_rows16(w, x, P, K, w.scalar_type(), "x");
@@ -414,6 +432,7 @@ std::tuple<OptTensor, OptTensor> expert_mm_backward(const Tensor& dz_in, const T
                                                     const Tensor& offsets, bool need_dx, bool need_dw,
                                                     const Tensor& err) {
   check_mm(w, offsets, err, "expert_linear_backward");
+  check_tangents(dz_in, x_in, w);
   const Tensor x = rows16(x_in), dz = rows16(dz_in);
   const int64_t P = x.size(0), N = w.size(1), K = w.size(2);
   check_rows16(w, x, P, K, w.scalar_type(), "x");
@@ -435,6 +454,7 @@ std::tuple<OptTensor, OptTensor> expert_mm_backward(const Tensor& dz_in, const T
 }
 
 Tensor swiglu_backward(const Tensor& da_in, const Tensor& pre_in, const Tensor& offsets) {
+  check_tangents(da_in, pre_in);
   const Tensor da = rows16(da_in), pre = rows16(pre_in);
   TORCH_CHECK(pre.is_cuda() && pre.dim() == 2 && is16(pre) && pre.size(1) >= 16 && pre.size(1) % 16 == 0,
               "swiglu_backward: pre must be a CUDA BF16 or FP16 [rows, n] tensor, n a multiple of 16");

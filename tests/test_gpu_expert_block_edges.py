@@ -172,3 +172,43 @@ def test_inplace_norm_and_operands_in_its_memory(cuda):
     want = fused.add_rmsnorm_mx(x.clone(), w, 1e-6, x.clone())
     new, codes, *_ = fused.add_rmsnorm_mx(x, w, 1e-6, x, inplace=True)  # x on itself
     assert torch.equal(new, want[0]) and torch.equal(codes, want[1])
+
+
+# ------------------------------------------------------------------------------------------------ tangents
+def test_tangents_are_refused(cuda):
+    """No operator has a forward-mode derivative: an input with a tangent is refused, not answered without one."""
+    from torch.autograd import forward_ad
+
+    g = gen(2)
+    x, w = randn(g, 6, 64, dtype=BF16), torch.ones(64, device="cuda")
+    d, df = randn(g, 6, 64, dtype=BF16), randn(g, 6, 64)
+    order = dispatch.expert_order(torch.arange(6, device="cuda").view(3, 2), 6)
+    weights, residual = torch.rand(3, 2, device="cuda", generator=g), randn(g, 3, 64, dtype=BF16)
+    mats = randn(g, 6, 32, 64, dtype=BF16)
+    dy, pre, da = randn(g, 6, 32, dtype=BF16), randn(g, 6, 64, dtype=BF16), randn(g, 6, 32, dtype=BF16)
+    calls = [
+        (lambda *t: fused.add_rmsnorm_mx(t[0], t[1], 1e-6, t[2], t[3]), (x, w, d, df)),
+        (lambda *t: fused.add_rmsnorm_mx(t[0].clone(), t[1], 1e-6, t[2], t[3], inplace=True), (x, w, d, df)),
+        (lambda *t: fused.add_rmsnorm_backward(t[0], t[1], t[2], 1e-6, t[3]), (d, x, w, d)),
+        (lambda t: dispatch.gather(t, order), (residual,)),
+        (lambda *t: dispatch.combine(t[0], order, t[1], t[2]), (x, weights, residual)),
+        (lambda *t: dispatch.combine_backward(t[0], t[1], order, t[2]), (residual, x, weights)),
+        (lambda *t: grouped.expert_linear(t[0], t[1], order.offsets), (x, mats)),
+        (lambda *t: grouped.expert_linear_backward(t[0], t[1], t[2], order.offsets), (dy, x, mats)),
+        (lambda *t: grouped.swiglu_backward(t[0], t[1], order.offsets), (da, pre)),
+    ]
+    for call, inputs in calls:
+        call(*inputs)
+        with forward_ad.dual_level():
+            call(*inputs)  # a level alone changes nothing
+            for i, t in enumerate(inputs):
+                dual = [forward_ad.make_dual(u, torch.ones_like(u)) if j == i else u for j, u in enumerate(inputs)]
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*dual)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*dual)
+    with forward_ad.dual_level():  # where a gradient is recorded too
+        dual = forward_ad.make_dual(residual.clone().requires_grad_(True), torch.ones_like(residual))
+        for call in (lambda t: dispatch.gather(t, order), lambda t: dispatch.combine(x, order, weights, t)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(dual)
