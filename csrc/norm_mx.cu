@@ -259,14 +259,16 @@ __global__ void __launch_bounds__(256) norm_dw_kernel(const float* __restrict__ 
   if (threadIdx.y == 0 && c < n) *reinterpret_cast<float4*>(dw + c) = s;
 }
 
-// code x 2^(scale - 127) in BF16 (exact: an E4M3 value has four significant bits).  Thread per 16 codes; memory bound.
+// code x 2^(scale - 127) in BF16: exact for scale bytes 3 to 246 (an E4M3 value has four significant bits), one rounding
+// beyond them, to zero, a subnormal or infinity; byte 255 is E8M0's NaN.  Thread per 16 codes; memory bound.
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint4* __restrict__ codes,
                                                             const uint8_t* __restrict__ scales, int64_t n16,
                                                             uint4* __restrict__ out) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= n16) return;
   const uint4 c = codes[i];
-  const float s = exp2f((float)scales[i >> 1] - 127.f);
+  const int e = scales[i >> 1];
+  const float s = e == 255 ? __int_as_float(0x7fffffff) : exp2f((float)(e - 127));
   const uint32_t w[4] = {c.x, c.y, c.z, c.w};
   uint32_t o[8];
 #pragma unroll

@@ -607,7 +607,7 @@ void bind_block_ops(pybind11::module_& m) {
   const auto unlocked = pybind11::call_guard<pybind11::gil_scoped_release>();
   m.def("add_rmsnorm_mx", &add_rmsnorm_mx_op, "residual add + RMSNorm -> MXFP8 rows", unlocked);
   m.def("rmsnorm_backward", &rmsnorm_backward, "gradient of residual add + RMSNorm", unlocked);
-  m.def("mx_dequantize", &mx_dequantize, "MXFP8 rows -> BF16 (exact)", unlocked);
+  m.def("mx_dequantize", &mx_dequantize, "MXFP8 rows -> BF16", unlocked);
   m.def("expert_order", &expert_order, "stable sort of (token, choice) pairs by expert", unlocked);
   m.def("expert_gather", &gather_op, "token rows -> rows sorted by expert", unlocked);
   m.def("expert_gather_mx", &expert_gather, "MXFP8 token rows -> rows sorted by expert", unlocked);

@@ -112,11 +112,13 @@ def mx_quantize(h: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """MXFP8 rows -> code x 2^(scale - 127).  Exact in BF16 and fp32 (E4M3 has four significant bits)."""
+    """MXFP8 rows -> code x 2^(scale - 127), NaN for scale byte 255.  E4M3 has four significant bits: exact for scale
+    bytes 3 to 246 in BF16 and 0 to 246 in fp32, rounded once beyond them (to zero, a subnormal or infinity)."""
     if codes.is_cuda and dtype == torch.bfloat16:
         return ext().mx_dequantize(codes, scales)
     v = codec.e4m3_decode(codes).unflatten(-1, (codes.shape[1] // MX_GROUP, MX_GROUP))
-    return (v * codec.exp2_int(scales.to(torch.int32) - 127)[..., None]).reshape(codes.shape).to(dtype)
+    s = torch.where(scales == 255, float("nan"), codec.exp2_int(scales.to(torch.int32) - 127))
+    return (v * s[..., None]).reshape(codes.shape).to(dtype)
 
 
 def _check_norm(x: torch.Tensor, w: torch.Tensor) -> None:

@@ -4,7 +4,7 @@ import torch
 
 import expert_block_reference as ref
 from expert_block_reference import ACC, F64
-from packmla.ops import grouped
+from packmla.ops import fused, grouped
 
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 
@@ -28,3 +28,18 @@ def test_rows_before_the_first_expert(table):
         ref.check(dw[e], dy[a:b].to(F64).T @ x[a:b].to(F64), (dy[a:b].to(F64).abs().T @ x[a:b].to(F64).abs()) * ACC * P, "dw")
     assert (grouped.expert_linear(x, w, offsets, activation="swiglu")[nobody] == 0).all()
     assert (grouped.swiglu_backward(dy[:, :N // 2], dy, offsets)[nobody] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,first", [(BF16, 3), (F32, 0)])
+def test_mx_dequantize_over_every_code_and_scale(dtype, first):
+    """code x 2^(scale - 127), rounded once where the type cannot hold it; scale byte 255 is NaN."""
+    codes = torch.arange(256, dtype=torch.uint8).repeat(256, 1)
+    scales = torch.arange(256, dtype=torch.uint8)[:, None].repeat(1, 8)
+    value = codes.view(torch.float8_e4m3fn).to(F64) * torch.exp2(torch.arange(256, dtype=F64) - 127)[:, None]
+    value[255] = float("nan")
+    want = value.float().to(dtype)
+    got = fused.mx_dequantize(codes, scales, dtype)
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
+    held = ~value[first:247].isnan()
+    assert torch.equal(want[first:247][held].to(F64), value[first:247][held])  # exact there

@@ -212,3 +212,18 @@ def test_tangents_are_refused(cuda):
         for call in (lambda t: dispatch.gather(t, order), lambda t: dispatch.combine(x, order, weights, t)):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call(dual)
+
+
+# ------------------------------------------------------------------------------------------------ MXFP8 values
+def test_mx_dequantize_over_every_code_and_scale(cuda):
+    """code x 2^(scale - 127), rounded once where BF16 cannot hold it (scale bytes 0 to 2 and from 247); 255 is NaN."""
+    codes = torch.arange(256, device="cuda", dtype=torch.uint8).repeat(256, 1)
+    scales = torch.arange(256, device="cuda", dtype=torch.uint8)[:, None].repeat(1, 8)
+    value = codes.view(torch.float8_e4m3fn).to(F64) * torch.exp2(torch.arange(256, device="cuda", dtype=F64) - 127)[:, None]
+    value[255] = float("nan")
+    want = value.float().bfloat16()
+    for got in (fused.mx_dequantize(codes, scales), fused.mx_dequantize(codes.cpu(), scales.cpu()).cuda()):
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
+    held = ~value[3:247].isnan()
+    assert torch.equal(want[3:247][held].to(F64), value[3:247][held])  # exact there
