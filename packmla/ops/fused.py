@@ -105,10 +105,15 @@ def _norm_oracle(s: torch.Tensor, w: torch.Tensor, eps: float):
 
 
 def mx_quantize(h: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """fp32 rows [T, n] -> (E4M3 codes [T, n], UE8M0 scale bytes [T, n / 32]), uint8: the rule of `add_rmsnorm_mx`."""
+    """fp32 rows [T, n] -> (E4M3 codes [T, n], UE8M0 scale bytes [T, n / 32]), uint8: the rule of `add_rmsnorm_mx`.
+
+    A NaN is a NaN code and counts for no scale; an infinity has the largest scale and code, which stand for infinity in
+    BF16 and fp32 (finite values beside it come out as zero)."""
     b = h.float().unflatten(-1, (h.shape[1] // MX_GROUP, MX_GROUP))
-    e = codec.ue8m0_exponent(b.abs().amax(-1))
-    return codec.e4m3_encode(b * codec.exp2_int(-e)[..., None]).reshape(h.shape), (e + 127).to(torch.uint8)
+    amax = torch.where(b.isnan(), 0.0, b.abs()).amax(-1)
+    e = codec.ue8m0_exponent(amax.clamp_max(torch.finfo(torch.float32).max))
+    codes = codec.e4m3_encode((b * codec.exp2_int(-e)[..., None]).clamp(-448, 448))
+    return codes.reshape(h.shape), (e + 127).to(torch.uint8)
 
 
 def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:

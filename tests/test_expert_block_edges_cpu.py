@@ -43,3 +43,22 @@ def test_mx_dequantize_over_every_code_and_scale(dtype, first):
     assert torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
     held = ~value[first:247].isnan()
     assert torch.equal(want[first:247][held].to(F64), value[first:247][held])  # exact there
+
+
+def test_mx_quantize_of_infinities_and_nan():
+    """Beside a NaN the finite values keep their codes and scale; infinities stay infinite."""
+    g = torch.Generator().manual_seed(1)
+    h = 3 * torch.randn(4, 96, generator=g)
+    codes, scales = fused.mx_quantize(h)
+    bad = h.clone()
+    bad[0, 5], bad[1, 40], bad[2, 70], bad[2, 71] = float("nan"), float("inf"), -float("inf"), float("nan")
+    bad[3] = float("nan")
+    got, gs = fused.mx_quantize(bad)
+    small = h[0, :32].abs().amax() == h[0, 5].abs()  # the NaN took the group's largest value away
+    assert not small and gs[0, 0] == scales[0, 0]
+    keep = torch.arange(96) != 5
+    assert torch.equal(got[0, keep], codes[0, keep]) and got[0, 5] & 127 == 127
+    v = fused.mx_dequantize(got, gs)
+    assert v[1, 40] == float("inf") and (v[1, 32:40] == 0).all() and torch.equal(got[1, :32], codes[1, :32])
+    assert v[2, 70] == -float("inf") and v[2, 71].isnan() and v[2, 72:].eq(0).all()
+    assert (got[3] & 127 == 127).all()

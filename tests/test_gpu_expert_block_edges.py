@@ -227,3 +227,17 @@ def test_mx_dequantize_over_every_code_and_scale(cuda):
         assert torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
     held = ~value[3:247].isnan()
     assert torch.equal(want[3:247][held].to(F64), value[3:247][held])  # exact there
+
+
+def test_rows_with_infinities_and_nan_match_the_host(cuda):
+    """Groups that hold infinities or NaN: finite values keep their codes beside a NaN, and infinities stay infinite."""
+    h = 1 + (torch.arange(96).float().view(1, 96) + 0.3) / 64
+    w = h[0].clone()
+    w[5], w[40], w[70], w[71] = float("nan"), float("inf"), -float("inf"), float("nan")
+    x = torch.ones(3, 96, dtype=BF16)
+    x[2, 9] = float("nan")
+    got = fused.add_rmsnorm_mx(x.cuda(), w.cuda(), 0.0)
+    want = fused.add_rmsnorm_mx(x, w, 0.0)
+    nan = want[1] & 127 == 127
+    assert torch.equal(got[1].cpu() & 127 == 127, nan) and torch.equal(got[1].cpu()[~nan], want[1][~nan])
+    assert torch.equal(got[2].cpu(), want[2])
