@@ -62,3 +62,17 @@ def test_mx_quantize_of_infinities_and_nan():
     assert v[1, 40] == float("inf") and (v[1, 32:40] == 0).all() and torch.equal(got[1, :32], codes[1, :32])
     assert v[2, 70] == -float("inf") and v[2, 71].isnan() and v[2, 72:].eq(0).all()
     assert (got[3] & 127 == 127).all()
+
+
+def test_requantizing_keeps_values_not_codes():
+    """What MXFP8 rows stand for is kept when quantized again; a maximum rounded down to 224 2^e takes the next smaller
+    scale then, and every code of its group changes."""
+    h = torch.zeros(2, 32)
+    h[0, 0], h[0, 1] = 225.0, 3.0
+    h[1] = torch.linspace(-300, 300, 32)
+    codes, scales = fused.mx_quantize(h)
+    values = fused.mx_dequantize(codes, scales)
+    again, smaller = fused.mx_quantize(values.float())
+    assert torch.equal(fused.mx_dequantize(again, smaller), values)
+    assert scales.tolist() == [[127], [127]] and smaller.tolist() == [[126], [127]]
+    assert (again[0, :2] != codes[0, :2]).all() and torch.equal(again[1], codes[1])
