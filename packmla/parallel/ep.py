@@ -83,7 +83,8 @@ class EPMoE:
         fp32 [T, H] = residual + sum_k w_k expert_k(row).  `local_fn` gets the values the rows stand for in BF16,
         which holds those of finite rows exactly: experts that quantize their inputs by the same rule (moe precision
         "default") compute with the same values (not always the same codes: a group whose maximum was rounded down to
-        224 x 2^e takes the next smaller scale).  A pair whose expert id is negative (a masked token) is not sent and adds nothing."""
+        224 x 2^e takes the next smaller scale).  A pair whose expert id is negative (a masked token) is not sent and
+        adds nothing."""
         T, k = topk_ids.shape
         masked = topk_ids < 0
         owner = torch.where(masked, -1, topk_ids // self.local_experts)

@@ -78,6 +78,22 @@ def test_experts_of_a_larger_table(cuda):
     check_errors(cuda)
 
 
+@pytest.mark.parametrize("K,N,dtype", [(64, 64, BF16), (136, 264, F16)])
+@pytest.mark.parametrize("bad", [[0, 500, 700], [-5, 80, 60], [90, 10, 160], [30, -3, 400], [900, 0, 7], [-9, -8, -7]])
+def test_wrong_tables_are_clamped(cuda, bad, K, N, dtype):
+    """A table that decreases or leaves the rows acts as its running maximum within them; no row around x or dy is read."""
+    P, pad = 160, 300
+    g = gen(K)
+    big_x = torch.full((P + 2 * pad, K), float("nan"), device="cuda", dtype=dtype)
+    big_dy = torch.full((P + 2 * pad, N), float("nan"), device="cuda", dtype=dtype)
+    x, dy = big_x[pad:pad + P], big_dy[pad:pad + P]
+    x.copy_(randn(g, P, K, dtype=dtype))
+    dy.copy_(randn(g, P, N, dtype=dtype))
+    w = randn(g, 2, N, K, dtype=dtype, scale=K ** -0.5)
+    offsets = torch.tensor(bad, dtype=torch.int32, device="cuda")
+    check_products(dy, x, w, offsets, offsets.clamp(0, P).cummax(0).values)
+
+
 # ------------------------------------------------------------------------------------------------ host threads
 def together(*calls, times=20000):
     """Every call from a thread and on a stream of its own, many times and closely interleaved; raises what any raised."""
@@ -241,3 +257,51 @@ def test_rows_with_infinities_and_nan_match_the_host(cuda):
     nan = want[1] & 127 == 127
     assert torch.equal(got[1].cpu() & 127 == 127, nan) and torch.equal(got[1].cpu()[~nan], want[1][~nan])
     assert torch.equal(got[2].cpu(), want[2])
+
+
+# ------------------------------------------------------------------------------------------------ paths
+def test_exchange_of_mx_rows_matches_the_host(cuda):
+    """`EPMoE.forward_mx` of one rank, its experts through the served path ("grouped" products), with masked tokens."""
+    from packmla.parallel.ep import EPMoE, local_expert_fn
+
+    g = torch.Generator().manual_seed(4)
+    T, E, k, H, I = 70, 6, 2, 128, 64
+    lw = {"w13": (torch.randn(E, 2 * I, H, generator=g) * H ** -0.5).to(BF16), "w2": (torch.randn(E, H, I, generator=g) * I ** -0.5).to(BF16)}
+    h = torch.randn(T, H, generator=g)
+    ids = torch.stack([torch.randperm(E, generator=g)[:k] for _ in range(T)]).int()
+    ids[::7] = -1
+    weights, residual = torch.rand(T, k, generator=g), torch.randn(T, H, generator=g)
+    codes, scales = fused.mx_quantize(h)
+    out = []
+    for dev in ("cpu", "cuda"):
+        ep = EPMoE(E)
+        fn = local_expert_fn({n: t.to(dev) for n, t in lw.items()}, 0, E, "bf16", precision="grouped")
+        out.append(ep.forward_mx(codes.to(dev), scales.to(dev), ids.to(dev), weights.to(dev), fn, residual.to(dev)).cpu())
+    check_errors(cuda)
+    assert torch.equal(out[1][::7], residual[::7])
+    # both sides round rows to BF16 at the same places; the products' sums differ in order
+    assert (out[1] - out[0]).norm() <= 2 ** -7 * (out[0] - residual).norm()
+
+
+def test_engine_with_grouped_experts_in_a_decode_graph(cuda):
+    """The grouped products in the served model: captured decode steps give the eager ones' tokens."""
+    from helpers import small_gpu_config
+    from packmla.config import EngineConfig
+    from packmla.engine.engine import Engine, SamplingParams
+    from packmla.models.weights import init_weights
+
+    cfg = small_gpu_config(expert_format="bf16")
+    W = init_weights(cfg, device=cuda, seed=7)
+    g = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(0, cfg.vocab_size, (n,), generator=g).tolist() for n in (90, 33)]
+    outs = []
+    for graphs in (False, True):
+        ecfg = EngineConfig(kv_cache_format="direct", max_running_requests=2, cuda_graph_bs=[1, 2], chunked_prefill_size=64,
+                            moe_precision="grouped", disable_cuda_graph=not graphs)
+        eng = Engine.build(cfg, ecfg, cuda, max_context=1024, max_requests=2, kv_bytes=64 << 20, weights=W)
+        if graphs:
+            eng.runner.capture()
+        outs.append(eng.generate(prompts, SamplingParams(max_new_tokens=6)))
+        eng.runner.release()
+    check_errors(cuda)
+    assert outs[0] == outs[1]
