@@ -645,12 +645,7 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, in
   }
   return true;
 }
-// Arrive on a barrier of any CTA of the cluster: releasing this thread's writes to the cluster, or (relaxed) only
-// counting, where what must be ordered is ordered by tcgen05 fences; a release waits for the thread's global
-// stores as well.
-__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar_cluster) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
-}
+// Arrive on a barrier of any CTA of the cluster, releasing this thread's accesses to the cluster.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }

@@ -463,7 +463,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
       if (!zero) {
         pm::tc_fence_before();
         __syncwarp();
-        if (lane == 0) pm::mbar_arrive_cluster_relaxed(pm::dsmem_addr(d_empty + buf, 0));
+        // released: the leader's next products into these columns come after the warp's reads of them
+        if (lane == 0) pm::mbar_arrive_cluster(pm::dsmem_addr(d_empty + buf, 0));
         buf ^= 1;
         if (buf == 0) dph ^= 1;
       }

@@ -94,6 +94,20 @@ def test_wrong_tables_are_clamped(cuda, bad, K, N, dtype):
     check_products(dy, x, w, offsets, offsets.clamp(0, P).cummax(0).values)
 
 
+def test_accumulators_handed_back_tile_after_tile(cuda):
+    """Many short tiles a CTA pair, each in the columns that the one before last left: the same bits every time."""
+    g = gen(9)
+    E, P, K, N = 64, 64 * 70 + 11, 64, 2048
+    offsets = (torch.arange(E + 1, device="cuda") * 70).int()
+    x, w = randn(g, P, K, dtype=BF16), randn(g, E, N, K, dtype=BF16, scale=K ** -0.5)
+    z, s = ref.linear(x, w, offsets)
+    want = grouped.expert_linear(x, w, offsets)
+    ref.check(want, z, s * ACC * K, "y")
+    for _ in range(200):
+        assert torch.equal(grouped.expert_linear(x, w, offsets), want)
+    check_errors(cuda)
+
+
 # ------------------------------------------------------------------------------------------------ host threads
 def together(*calls, times=20000):
     """Every call from a thread and on a stream of its own, many times and closely interleaved; raises what any raised."""
