@@ -20,8 +20,9 @@ constexpr int kTileK = 64;         // of the reduced dimension per stage: 128 by
 constexpr int kMaxStages = 8;
 enum Mode { kForward = 0, kGradX = 1, kGradW = 2 };
 
-// Fast division (within 2 units in the last place, far below the outputs' rounding): the full one's extra
-// instructions lengthened the gated epilogue by half.  A denominator beyond 2^126, infinity included, gives 0.
+// Fast division and exponential: the full ones' extra instructions lengthened the gated epilogue by half.  The division
+// is within 2 units in the last place; the exponential's bound grows with |g| (2 + 1.17 |g| units), to 2^-16 of it where
+// it leaves fp32: far below the outputs' rounding (2^-8 BF16, 2^-11 FP16).  A denominator beyond 2^126, infinity included, gives 0.
 __device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
 __device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.f + __expf(-g)); }
 
@@ -479,6 +480,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair_threads(MODE), 
 
 // ----------------------------------------------------------------------------- SwiGLU gradient
 // da = gradient of silu(g) u; z = [g | u] rows: dg = da u s (1 + g (1 - s)), du = da g s with s = sigmoid(g).
+// dz is rounded to 16 bits because the products dx and dw take it as a tensor core operand, as z was when it was kept: the
+// error of dx and dw is that of two roundings (0.0023 of their norm with BF16, 0.0017 with an fp32 dz).
 // Rows before offsets[0] and past offsets[E] are zero.  Memory bound: 6 bytes read and 4 written per value of da; a block per row (58 us
 // for 16384 x 2048, 5.8 TB/s; walking blocks 61 us).
 template <typename T>

@@ -291,8 +291,9 @@ dim3 norm_block(int n, int vpt) {
   const int ty = tx >= 256 ? 1 : 256 / tx;
   return dim3(tx, ty);
 }
-// Vectors of a thread by width: one up to 4096 columns (2.7 us for 8 rows of 4096 against 3.6 with two, half the serial
-// work of a thread; 27.2 for 4999 rows of 2080 against 29.5; 74 for 8192 of 4096, 5.9 TB/s, against 72), two beyond.
+// Vectors of a thread by width, two past 4096 columns and one up to there: half the serial work of a thread (2.7 us for
+// 8 rows of 4096 against 3.6 with two; 27.2 for 4999 rows of 2080 against 29.5).  Many rows of 4096 would take two 3 %
+// better (8192: 74 us, 5.9 TB/s, against 72): the rule looks at the width alone.
 template <int VPT>
 void launch_fwd(const NormMxArgs& a, cudaStream_t stream) {
   const dim3 block = norm_block(a.n, VPT);

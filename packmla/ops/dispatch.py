@@ -18,11 +18,12 @@ from torch.autograd.function import once_differentiable
 
 from ._ext import ext
 
-MAX_EXPERTS = 4096
+MAX_EXPERTS = 4096  # of a sort; the products of ops/grouped.py take 1024 on CUDA
 
 
 class ExpertOrder(NamedTuple):
-    """Rows sorted by expert, earlier pairs first.  A pair whose expert is not in [base, base + E) - masked
+    """Rows sorted by expert, earlier pairs first, as `expert_order` makes them (a slice of offsets is for the products
+    alone: `gather` and `combine` go by the whole table).  A pair whose expert is not in [base, base + E) - masked
     tokens use -1 - has no row.  Rows past offsets[E] belong to no pair."""
 
     offsets: torch.Tensor  # int32 [E + 1]: expert e owns rows offsets[e] .. offsets[e + 1]

@@ -4,7 +4,11 @@ Rows are sorted by expert (`ops/dispatch.py`): expert e owns rows offsets[e] .. 
 weight is w[e] [N, K] (K contiguous, the convention of the model's `w13` = [gate rows | up rows] and `w2`).
 The offsets ascend and stay on the device.  Rows before offsets[0] and past offsets[E] give zero rows, so a slice
 offsets[a : b + 1] with w[a : b] computes some of a larger table's experts.  CUDA: csrc/expert_mm.cu (tcgen05, BF16
-or FP16 operands, fp32 accumulators, one rounding); CPU tensors: the same products in fp32.
+or FP16 operands, fp32 accumulators, one rounding), at most 1024 experts a call (the tile table lies in shared memory);
+CPU tensors: the same products in fp32.
+
+The tensor cores take 16-bit operands: a gated product keeps its operands for the backward pass in x's type, and their
+gradient is rounded to it before dx and dw are formed from it.
 """
 from __future__ import annotations
 
@@ -104,7 +108,7 @@ def expert_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, activ
 
     x [P, K] and w [E, N, K] BF16 or FP16 (N, K multiples of 8; N of 16 with "swiglu"), offsets int32 [E + 1] on the
     same device.  Differentiable in x and w: a gated product keeps its [P, N] operands, rounded to x's type, for
-    the backward pass."""
+    the backward pass, and rounds their gradient likewise."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {ACTIVATIONS}")
     _check(x, w, offsets, w.shape[2] if w.dim() == 3 else 0, "x")
